@@ -282,6 +282,119 @@ hipError_t gdn_causal_conv1d_update(const void* x, void* conv_state, const void*
                                     int64_t y_bstride, int64_t y_tstride, int64_t y_dstride,
                                     int io_dtype, int w_dtype, int silu, hipStream_t stream);
 
+/* ---- State-space layers (no counterpart in the reference) ----------------
+ * The other recurrent mixer that sits between the causal conv1d and a gated
+ * norm.  Per head h of `heads`, with state S fp32 [state_dim][head_dim] and B,
+ * C of group h / (heads / groups), token by token:
+ *   d = clamp(softplus(dt + dt_bias), dt_min, dt_max),  a = exp(-exp(A_log) d)
+ *   S <- a S + (d B) x^T,    y = (S^T C + D x) silu(z)
+ * The tensors a caller passes, device memory except the struct itself, which
+ * is read before the call returns:
+ *   x, z : [batch][tokens][heads][head_dim] of io_dtype, z may be null (no gate)
+ *   b, c : [batch][tokens][groups][state_dim] of io_dtype
+ *   dt   : [batch][tokens][heads] of dt_dtype (io_dtype or fp32)
+ *   A_log: fp32 [heads]; D, dt_bias: fp32 [heads] or null (zeros)
+ * A row's heads (groups) lie next to each other; batches and tokens lie
+ * *_batch and *_token elements apart (token strides below 2^31).  x, z, b, c
+ * are 16-byte aligned with strides that are multiples of 8.  head_dim is a
+ * multiple of 16 up to 256, state_dim 16, 32, 64, 128 or 256, 0 <= dt_min <=
+ * dt_max.  A token whose inputs are not finite leaves undefined values in its
+ * sequence from the 64-token chunk that holds it on. */
+typedef struct {
+    const void *x, *dt, *b, *c, *z;
+    const float *A_log, *D, *dt_bias;
+    int64_t x_batch, x_token, dt_batch, dt_token, b_batch, b_token, c_batch, c_token, z_batch,
+        z_token;
+    int batch, tokens, heads, head_dim, groups, state_dim, io_dtype, dt_dtype;
+    float dt_min, dt_max;
+} gdn_ssm_inputs;
+
+/* Decode: `tokens` >= 0 tokens of every batch row, y packed [batch][tokens]
+ * [heads][head_dim] (8-byte aligned), the state updated in place.  slots null:
+ * state is [batch][heads][state_dim][head_dim].  slots int32 [batch]: state is
+ * a pool of num_slots such states and row b uses state slots[b]; a slot
+ * outside [0, num_slots) is a row without a request: its y rows are zeros and
+ * no state changes.  Two rows of a call must not name one slot (their results
+ * would be undefined, in bounds). */
+hipError_t gdn_ssm_step(const gdn_ssm_inputs* in, void* y, float* state, const int32_t* slots,
+                        int num_slots, hipStream_t stream);
+
+/* Prompts.  cu_seqlens null: `batch` sequences of `tokens` tokens (num_seqs is
+ * batch).  cu_seqlens int32 [num_seqs + 1]: batch is 1 and the row holds
+ * packed sequences (clamped as in deltanet_chunk_prefill_varlen; y rows behind
+ * the last sequence are not written).  s0 (or null: zeros) and sf are fp32
+ * [num_seqs][heads][state_dim][head_dim]; sf may be s0.  A sequence without
+ * tokens hands its state on.  blocks (or null): gdn_request_blocks' table for
+ * the same cu_seqlens and this `block`; without it a packed call forms the
+ * table itself in the workspace.  `block` is the run of tokens that is worked
+ * on at a time, a multiple of 64, normally gdn_ssm_scan_block's; results for
+ * different blocks differ by rounding.  The workspace is 256-byte aligned,
+ * gdn_ssm_scan_workspace_size bytes (0: unsupported arguments). */
+int gdn_ssm_scan_block(const gdn_ssm_inputs* in, int num_seqs);
+size_t gdn_ssm_scan_workspace_size(const gdn_ssm_inputs* in, int num_seqs, int block, int packed);
+hipError_t gdn_ssm_scan(const gdn_ssm_inputs* in, void* y, const float* s0, float* sf,
+                        const int32_t* cu_seqlens, const int32_t* blocks, int num_seqs, int block,
+                        void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Tables of a packed batch from request lengths (device int32 [num_requests];
+ * negative ones count as 0, and what passes total_tokens is cut off):
+ *   cu_seqlens  int32 [num_requests + 1]
+ *   blocks      int32 [rows][4], rows = gdn_request_block_rows(...): request,
+ *               first token, tokens (at most `block`) and index within the
+ *               request of each block, in order, one empty block for a request
+ *               without tokens; (-1, 0, 0, 0) past the last block
+ *   token_slots int32 [total_tokens]: slots[request] (slots null: the request)
+ *   token_pos   int32 [total_tokens]: position within the request
+ *               (-1 and 0 behind the last request)
+ *   row_start   int32 [num_requests + 1], scratch
+ * block is a multiple of 64; total_tokens <= 2^30, num_requests <= 2^24;
+ * blocks, token_slots and token_pos 16-byte aligned.  gdn_request_block_rows
+ * is a host function: total_tokens / block + num_requests, or 0 for
+ * unsupported sizes. */
+int gdn_request_block_rows(int total_tokens, int num_requests, int block);
+hipError_t gdn_request_blocks(const int32_t* lengths, const int32_t* slots, int num_requests,
+                              int total_tokens, int block, int32_t* cu_seqlens,
+                              int32_t* row_start, int32_t* blocks, int32_t* token_slots,
+                              int32_t* token_pos, hipStream_t stream);
+
+/* gdn_causal_conv1d_fwd that continues from a state and hands one on, for
+ * fixed-length or packed sequences.  x, y, w, bias, K, dtypes and silu as
+ * there; state0 (or null: zeros) and state are [num_seqs][D][state_len] of
+ * io_dtype, oldest token first, state_len in K-1..8, 16-byte aligned; state
+ * (out) holds the last state_len tokens of state0 followed by the sequence, and
+ * must not be state0.  cu_seqlens (B = 1) as in gdn_ssm_scan, or null
+ * (num_seqs is B); y rows behind the last sequence are not written.  The sum
+ * stays in fp32 up to the one rounding of y. */
+hipError_t gdn_causal_conv1d_prefill(const void* x, const void* w, const void* bias,
+                                     const void* state0, void* y, void* state, int B, int T,
+                                     int D, int K, int state_len, int64_t x_bstride,
+                                     int64_t x_tstride, int64_t y_bstride, int64_t y_tstride,
+                                     const int32_t* cu_seqlens, int num_seqs, int io_dtype,
+                                     int w_dtype, int silu, hipStream_t stream);
+
+/* Gated norm over groups of a row of C channels, for rows longer than
+ * gdn_gated_rmsnorm_forward's: with u = x silu(z) (gate_first) or u = x,
+ *   y = u rsqrt(mean over the group of u^2 + eps) w  [silu(z) unless gate_first]
+ * in fp32, rounded once.  x, z: rows x_row and z_row elements apart
+ * (multiples of 8, 16-byte aligned); y packed; w: io_dtype or fp32 [C].
+ * C / groups a multiple of 8 up to 16384. */
+hipError_t gdn_gated_groupnorm_forward(const void* x, int64_t x_row, const void* z, int64_t z_row,
+                                       const void* w, void* y, int64_t rows, int C, int groups,
+                                       float eps, int gate_first, int io_dtype, int w_dtype,
+                                       hipStream_t stream);
+
+/* gdn_causal_conv1d_update on a pool of num_slots conv states: row b uses
+ * state slots[b] (device int32 [B]); a slot outside the pool is a row without
+ * a request: its y is zero and no state changes. */
+hipError_t gdn_causal_conv1d_update_slots(const void* x, void* conv_state, const void* w,
+                                          const void* bias, void* y, const int32_t* slots,
+                                          int num_slots, int B, int T, int D, int K,
+                                          int state_len, int64_t x_bstride, int64_t x_tstride,
+                                          int64_t x_dstride, int64_t s_bstride, int64_t s_dstride,
+                                          int64_t y_bstride, int64_t y_tstride, int64_t y_dstride,
+                                          int io_dtype, int w_dtype, int silu,
+                                          hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

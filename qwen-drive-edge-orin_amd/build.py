@@ -23,7 +23,8 @@ INCLUDE = REPO / "include"
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 HIP_SOURCES = ["gdn_prefill.hip", "gdn_decode.hip", "gated_rmsnorm.hip", "causal_conv1d.hip",
-               "stream_probe.hip"]
+               "causal_conv1d_prefill.hip", "ssm_scan.hip", "ssm_step.hip", "request_blocks.hip",
+               "gated_groupnorm.hip", "stream_probe.hip"]
 LIB_NAME = "libgdn_hip.so"
 EXT_NAME = "deltanet_chunk_hip"
 
@@ -73,7 +74,7 @@ def build_ext() -> Path:
            f"-DTORCH_EXTENSION_NAME={EXT_NAME}", "-DTORCH_API_INCLUDE_EXTENSION_H",
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            *[f"-I{p}" for p in incs],
-           str(CSRC / "torch_binding.cpp"),
+           str(CSRC / "torch_binding.cpp"), str(CSRC / "torch_ssm.cpp"),
            f"-L{OUT}", "-lgdn_hip",
            *[f"-L{p}" for p in libdirs],
            "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python",

@@ -254,7 +254,7 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv1d_update_kernel(
     const uint16_t* __restrict__ x, uint16_t* __restrict__ state, const void* __restrict__ w,
     const void* __restrict__ bias, uint16_t* __restrict__ y, int B, int T, int D, int state_len,
     int64_t xbs, int64_t xts, int64_t xds, int64_t sbs, int64_t sds, int64_t ybs, int64_t yts,
-    int64_t yds) {
+    int64_t yds, const int32_t* __restrict__ slots, int num_slots) {
     const int64_t gid = (int64_t)blockIdx.x * kConvThreads + threadIdx.x;
     if (gid >= (int64_t)B * D) return;
     const int b = (int)(gid / D), d = (int)(gid - (int64_t)b * D);
@@ -262,7 +262,15 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv1d_update_kernel(
 #pragma unroll
     for (int j = 0; j < K; ++j) wf[j] = ld_elem<WT>(w, (size_t)d * K + j);
     const float bv = bias ? ld_elem<WT>(bias, d) : 0.f;   // added only with a bias
-    uint16_t* st = state + (size_t)b * sbs + (size_t)d * sds;
+    int slot = b;
+    if (slots) {   // a pool of states: row b uses slots[b], none outside the pool
+        slot = slots[b];
+        if (slot < 0 || slot >= num_slots) {
+            for (int i = 0; i < T; ++i) y[(size_t)b * ybs + (size_t)d * yds + (size_t)i * yts] = 0;
+            return;
+        }
+    }
+    uint16_t* st = state + (size_t)slot * sbs + (size_t)d * sds;
     const uint16_t* xs = x + (size_t)b * xbs + (size_t)d * xds;
     uint16_t* ys = y + (size_t)b * ybs + (size_t)d * yds;
     // the old state (one 8-byte access for the common 4-token row), then a
@@ -343,11 +351,21 @@ template <int IO, int WT, bool SILU>
 __global__ __launch_bounds__(kUpd4Threads) void causal_conv1d_update4_kernel(
     const uint16_t* __restrict__ x, uint16_t* __restrict__ state, const void* __restrict__ w,
     const void* __restrict__ bias, uint16_t* __restrict__ y, int B, int T, int D, int64_t xbs,
-    int64_t xts, int64_t sbs, int64_t ybs, int64_t yts) {
+    int64_t xts, int64_t sbs, int64_t ybs, int64_t yts, const int32_t* __restrict__ slots,
+    int num_slots) {
     const int64_t gid = (int64_t)blockIdx.x * kUpd4Threads + threadIdx.x;
     const int D4 = D / 4;
     if (gid >= (int64_t)B * D4) return;
     const int b = (int)(gid / D4), d0 = 4 * (int)(gid - (int64_t)b * D4);
+    int slot = b;
+    if (slots) {   // as above
+        slot = slots[b];
+        if (slot < 0 || slot >= num_slots) {
+            for (int i = 0; i < T; ++i)
+                *reinterpret_cast<uint2*>(y + (size_t)b * ybs + d0 + (size_t)i * yts) = make_uint2(0, 0);
+            return;
+        }
+    }
     // weights [d0 .. d0+3][0..3] and bias
     float wf[4][4], bv[4] = {0.f, 0.f, 0.f, 0.f};
     if constexpr (WT == 2) {
@@ -388,7 +406,7 @@ __global__ __launch_bounds__(kUpd4Threads) void causal_conv1d_update4_kernel(
     __builtin_assume(T >= 1);
     uint2 xr = *reinterpret_cast<const uint2*>(xb);
     // state rows: channel e's 4 tokens, oldest first, 8 bytes per channel
-    uint16_t* st = state + (size_t)b * sbs + (size_t)d0 * 4;
+    uint16_t* st = state + (size_t)slot * sbs + (size_t)d0 * 4;
     uint16_t win[4][4];   // [channel][slot]: the last 4 window tokens, oldest first
     {
         const u32x4 r0 = reinterpret_cast<const u32x4*>(st)[0];   // channels 0, 1
@@ -546,7 +564,8 @@ template <int IO, int WT>
 hipError_t launch_update(const void* x, void* state, const void* w, const void* bias, void* y,
                          int B, int T, int D, int K, int state_len, int64_t xbs, int64_t xts,
                          int64_t xds, int64_t sbs, int64_t sds, int64_t ybs, int64_t yts,
-                         int64_t yds, int silu, hipStream_t stream) {
+                         int64_t yds, int silu, const int32_t* slots, int num_slots,
+                         hipStream_t stream) {
     // the vector path: K = 4, 4-token state rows, unit channel strides, and
     // every vector access aligned (x, y: 8 bytes per 4 channels; state and
     // weights: 16; bias: 8, or 16 in fp32)
@@ -554,7 +573,8 @@ hipError_t launch_update(const void* x, void* state, const void* w, const void* 
         return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
     };
     if (K == 4 && state_len == 4 && sds == 4 && xds == 1 && yds == 1 && D % 4 == 0 &&
-        (B <= 1 || (xbs % 4 == 0 && ybs % 4 == 0 && sbs % 8 == 0)) &&
+        (B <= 1 || (xbs % 4 == 0 && ybs % 4 == 0)) &&
+        ((B <= 1 && !slots) || sbs % 8 == 0) &&
         (T <= 1 || (xts % 4 == 0 && yts % 4 == 0)) && al(x, 8) && al(y, 8) && al(state, 16) &&
         al(w, 16) && (!bias || al(bias, WT == 2 ? 16 : 8))) {
         const int64_t n4 = (int64_t)B * (D / 4);
@@ -562,15 +582,15 @@ hipError_t launch_update(const void* x, void* state, const void* w, const void* 
         auto xp = static_cast<const uint16_t*>(x);
         auto sp = static_cast<uint16_t*>(state);
         auto yp = static_cast<uint16_t*>(y);
-        const int64_t xb = B <= 1 ? 0 : xbs, yb = B <= 1 ? 0 : ybs, sb = B <= 1 ? 0 : sbs;
+        const int64_t xb = B <= 1 ? 0 : xbs, yb = B <= 1 ? 0 : ybs, sb = B <= 1 && !slots ? 0 : sbs;
         if (silu)
             hipLaunchKernelGGL((causal_conv1d_update4_kernel<IO, WT, true>), grid4,
                                dim3(kUpd4Threads), 0, stream, xp, sp, w, bias, yp, B, T, D, xb,
-                               xts, sb, yb, yts);
+                               xts, sb, yb, yts, slots, num_slots);
         else
             hipLaunchKernelGGL((causal_conv1d_update4_kernel<IO, WT, false>), grid4,
                                dim3(kUpd4Threads), 0, stream, xp, sp, w, bias, yp, B, T, D, xb,
-                               xts, sb, yb, yts);
+                               xts, sb, yb, yts, slots, num_slots);
         return hipGetLastError();
     }
     const int64_t n = (int64_t)B * D;
@@ -583,11 +603,13 @@ hipError_t launch_update(const void* x, void* state, const void* w, const void* 
         if (silu)                                                                               \
             hipLaunchKernelGGL((causal_conv1d_update_kernel<IO, WT, KK, true>), grid,          \
                                dim3(kConvThreads), 0, stream, xp, sp, w, bias, yp, B, T, D,     \
-                               state_len, xbs, xts, xds, sbs, sds, ybs, yts, yds);              \
+                               state_len, xbs, xts, xds, sbs, sds, ybs, yts, yds, slots,        \
+                               num_slots);                                                      \
         else                                                                                    \
             hipLaunchKernelGGL((causal_conv1d_update_kernel<IO, WT, KK, false>), grid,         \
                                dim3(kConvThreads), 0, stream, xp, sp, w, bias, yp, B, T, D,     \
-                               state_len, xbs, xts, xds, sbs, sds, ybs, yts, yds);              \
+                               state_len, xbs, xts, xds, sbs, sds, ybs, yts, yds, slots,        \
+                               num_slots);                                                      \
         break;
     switch (K) {
         GDN_CONV_UPD(2)
@@ -630,14 +652,13 @@ extern "C" hipError_t gdn_causal_conv1d_fwd(const void* x, const void* w, const 
 #undef GDN_FWD_ARGS
 }
 
-extern "C" hipError_t gdn_causal_conv1d_update(const void* x, void* conv_state, const void* w,
-                                               const void* bias, void* y, int B, int T, int D,
-                                               int K, int state_len, int64_t x_bstride,
-                                               int64_t x_tstride, int64_t x_dstride,
-                                               int64_t s_bstride, int64_t s_dstride,
-                                               int64_t y_bstride, int64_t y_tstride,
-                                               int64_t y_dstride, int io_dtype, int w_dtype,
-                                               int silu, hipStream_t stream) {
+namespace {
+hipError_t update_entry(const void* x, void* conv_state, const void* w, const void* bias, void* y,
+                        int B, int T, int D, int K, int state_len, int64_t x_bstride,
+                        int64_t x_tstride, int64_t x_dstride, int64_t s_bstride,
+                        int64_t s_dstride, int64_t y_bstride, int64_t y_tstride,
+                        int64_t y_dstride, int io_dtype, int w_dtype, int silu,
+                        const int32_t* slots, int num_slots, hipStream_t stream) {
     if (B < 0 || T < 0 || D <= 0 || K < 2 || K > 4) return hipErrorInvalidValue;
     if (state_len < K - 1 || state_len > kConvMaxState) return hipErrorInvalidValue;
     if (!conv_dtypes_ok(io_dtype, w_dtype) || (silu != 0 && silu != 1)) return hipErrorInvalidValue;
@@ -647,8 +668,34 @@ extern "C" hipError_t gdn_causal_conv1d_update(const void* x, void* conv_state, 
     const bool bf = io_dtype == GDN_DTYPE_BF16, w32 = w_dtype == GDN_DTYPE_FP32;
 #define GDN_UPD_ARGS                                                                             \
     x, conv_state, w, bias, y, B, T, D, K, state_len, x_bstride, x_tstride, x_dstride, s_bstride, \
-        s_dstride, y_bstride, y_tstride, y_dstride, silu, stream
+        s_dstride, y_bstride, y_tstride, y_dstride, silu, slots, num_slots, stream
     if (bf) return w32 ? launch_update<0, 2>(GDN_UPD_ARGS) : launch_update<0, 0>(GDN_UPD_ARGS);
     return w32 ? launch_update<1, 2>(GDN_UPD_ARGS) : launch_update<1, 1>(GDN_UPD_ARGS);
 #undef GDN_UPD_ARGS
+}
+}  // namespace
+
+extern "C" hipError_t gdn_causal_conv1d_update(const void* x, void* conv_state, const void* w,
+                                               const void* bias, void* y, int B, int T, int D,
+                                               int K, int state_len, int64_t x_bstride,
+                                               int64_t x_tstride, int64_t x_dstride,
+                                               int64_t s_bstride, int64_t s_dstride,
+                                               int64_t y_bstride, int64_t y_tstride,
+                                               int64_t y_dstride, int io_dtype, int w_dtype,
+                                               int silu, hipStream_t stream) {
+    return update_entry(x, conv_state, w, bias, y, B, T, D, K, state_len, x_bstride, x_tstride,
+                        x_dstride, s_bstride, s_dstride, y_bstride, y_tstride, y_dstride, io_dtype,
+                        w_dtype, silu, nullptr, 0, stream);
+}
+
+extern "C" hipError_t gdn_causal_conv1d_update_slots(
+    const void* x, void* conv_state, const void* w, const void* bias, void* y,
+    const int32_t* slots, int num_slots, int B, int T, int D, int K, int state_len,
+    int64_t x_bstride, int64_t x_tstride, int64_t x_dstride, int64_t s_bstride, int64_t s_dstride,
+    int64_t y_bstride, int64_t y_tstride, int64_t y_dstride, int io_dtype, int w_dtype, int silu,
+    hipStream_t stream) {
+    if (!slots || num_slots < 1) return hipErrorInvalidValue;
+    return update_entry(x, conv_state, w, bias, y, B, T, D, K, state_len, x_bstride, x_tstride,
+                        x_dstride, s_bstride, s_dstride, y_bstride, y_tstride, y_dstride, io_dtype,
+                        w_dtype, silu, slots, num_slots, stream);
 }

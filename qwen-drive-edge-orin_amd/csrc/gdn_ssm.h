@@ -1,0 +1,59 @@
+// What the state-space kernels share: the argument struct's device view, the
+// step size and decay of a token, and the host checks.
+#pragma once
+
+#include "gdn_common.h"
+#include "gdn_hip.h"
+#include "gdn_io.h"
+
+#include <math.h>
+
+namespace gdn {
+
+// d = clamp(softplus(raw + bias), lo, hi); the large branch keeps e^x finite
+__device__ __forceinline__ float ssm_delta(float raw, float bias, float lo, float hi) {
+    const float x = raw + bias;
+    const float d = x > 20.f ? x : log1pf(expf(x));
+    return fminf(fmaxf(d, lo), hi);
+}
+
+inline bool ssm_aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// Row strides that every 16-byte lane access of x, B, C and z needs
+inline bool ssm_rows_ok(const void* p, int64_t batch, int64_t token) {
+    return p && ssm_aligned(p, 16) && batch >= 0 && token >= 0 && token <= 0x7fffffff &&
+           batch % 8 == 0 && token % 8 == 0;
+}
+
+// The sizes of gdn_ssm_inputs
+inline bool ssm_sizes_ok(const gdn_ssm_inputs* a) {
+    if (!a || a->batch < 1 || a->tokens < 0 || a->heads < 1 || a->groups < 1 ||
+        a->heads % a->groups != 0)
+        return false;
+    if (a->head_dim < 16 || a->head_dim > 256 || a->head_dim % 16 != 0) return false;
+    if (a->state_dim != 16 && a->state_dim != 32 && a->state_dim != 64 && a->state_dim != 128 &&
+        a->state_dim != 256)
+        return false;
+    return true;
+}
+
+// Sizes, types and pointers
+inline bool ssm_inputs_ok(const gdn_ssm_inputs* a) {
+    if (!ssm_sizes_ok(a)) return false;
+    if (a->io_dtype != GDN_DTYPE_BF16 && a->io_dtype != GDN_DTYPE_FP16) return false;
+    if (a->dt_dtype != a->io_dtype && a->dt_dtype != GDN_DTYPE_FP32) return false;
+    if (!(a->dt_min >= 0.f) || !(a->dt_max >= a->dt_min)) return false;
+    if (a->tokens == 0) return true;
+    if (!ssm_rows_ok(a->x, a->x_batch, a->x_token) || !ssm_rows_ok(a->b, a->b_batch, a->b_token) ||
+        !ssm_rows_ok(a->c, a->c_batch, a->c_token) || !a->dt || !a->A_log || a->dt_batch < 0 ||
+        a->dt_token < 0 || a->dt_token > 0x7fffffff)
+        return false;
+    return !a->z || ssm_rows_ok(a->z, a->z_batch, a->z_token);
+}
+
+// The recurrence over whole sequences, one wave per 32 columns of a head
+// (ssm_step.hip): s0 null is zeros, s0 may be sf
+hipError_t ssm_recurrent(const gdn_ssm_inputs& in, void* y, const float* s0, float* sf,
+                         const int32_t* cu, int seqs, hipStream_t stream);
+
+}  // namespace gdn

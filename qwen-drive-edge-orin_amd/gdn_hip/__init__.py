@@ -21,8 +21,26 @@ The compiled pieces live next to this file:
                           raw q/k/v and gate inputs     (state updated in place)
   gated_rmsnorm(x, z, weight, eps=1e-6) -> y
   causal_conv1d_fwd(x, weight, bias=None, silu=False) -> y      x, y [B, D, T]
-  causal_conv1d_update(x, conv_state, weight, bias=None, silu=False) -> y
+  causal_conv1d_update(x, conv_state, weight, bias=None, silu=False, *, slots=None) -> y
                                                   (conv_state updated in place)
+
+State-space layers (x, z [B, T, H, P], dt [B, T, H], B, C [B, T, G, N], states
+fp32 [B, H, N, P]; A_log, D, dt_bias fp32 [H]):
+
+  ssm_scan(x, dt, A_log, B, C, D=None, z=None, dt_bias=None, s0=None, *,
+           cu_seqlens=None, blocks=None, block=0, dt_min=0, dt_max=inf) -> [y, final_state]
+  ssm_step(x, dt, A_log, B, C, state, D=None, z=None, dt_bias=None, *, slots=None,
+           dt_min=0, dt_max=inf) -> y             (state updated in place)
+  causal_conv1d_prefill(x, weight, bias=None, state0=None, *, silu=False,
+                        cu_seqlens=None, state_len=0) -> [y [B, D, T], state [N, D, L]]
+  request_blocks(lengths, total_tokens, *, block=64, slots=None)
+                          -> [cu_seqlens, blocks, token_slots, token_pos]
+  ssm_scan_block(tokens, batch, heads, head_dim, groups, state_dim, num_seqs) -> block
+                          for request_blocks, whose table several scans may share
+  gated_groupnorm(x, z, weight, groups, eps=1e-6, *, gate_first=True) -> y
+
+slots [B]: the states are a pool and row b uses state slots[b]; a slot outside
+the pool is a row without a request (zeros, no state changes).
 
 ``checked=True`` synchronises after the call and raises when one of the
 scan's bounded waits gave up (o and the state would then be incomplete);
@@ -34,6 +52,7 @@ Build with ``python qwen-drive-edge-orin_amd/build.py``.
 from __future__ import annotations
 
 import importlib
+import math
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -97,5 +116,35 @@ def causal_conv1d_fwd(x, weight, bias=None, silu=False):
     return load().causal_conv1d_fwd(x, weight, bias, silu)
 
 
-def causal_conv1d_update(x, conv_state, weight, bias=None, silu=False):
-    return load().causal_conv1d_update(x, conv_state, weight, bias, silu)
+def causal_conv1d_update(x, conv_state, weight, bias=None, silu=False, *, slots=None):
+    return load().causal_conv1d_update(x, conv_state, weight, bias, silu, slots=slots)
+
+
+def ssm_scan(x, dt, A_log, B, C, D=None, z=None, dt_bias=None, s0=None, *, cu_seqlens=None,
+             blocks=None, block=0, dt_min=0.0, dt_max=math.inf):
+    return load().ssm_scan(x, dt, A_log, B, C, D, z, dt_bias, s0, cu_seqlens=cu_seqlens,
+                           blocks=blocks, block=block, dt_min=dt_min, dt_max=dt_max)
+
+
+def ssm_scan_block(tokens, batch, heads, head_dim, groups, state_dim, num_seqs):
+    return load().ssm_scan_block(tokens, batch, heads, head_dim, groups, state_dim, num_seqs)
+
+
+def ssm_step(x, dt, A_log, B, C, state, D=None, z=None, dt_bias=None, *, slots=None, dt_min=0.0,
+             dt_max=math.inf):
+    return load().ssm_step(x, dt, A_log, B, C, state, D, z, dt_bias, slots=slots, dt_min=dt_min,
+                           dt_max=dt_max)
+
+
+def causal_conv1d_prefill(x, weight, bias=None, state0=None, *, silu=False, cu_seqlens=None,
+                          state_len=0):
+    return load().causal_conv1d_prefill(x, weight, bias, state0, silu=silu, cu_seqlens=cu_seqlens,
+                                        state_len=state_len)
+
+
+def request_blocks(lengths, total_tokens, *, block=64, slots=None):
+    return load().request_blocks(lengths, total_tokens, block=block, slots=slots)
+
+
+def gated_groupnorm(x, z, weight, groups, eps=1e-6, *, gate_first=True):
+    return load().gated_groupnorm(x, z, weight, groups, eps, gate_first=gate_first)

@@ -25,7 +25,34 @@ HIP_ERROR_INVALID_VALUE = 1
 HIP_ERROR_LAUNCH_TIMEOUT = 702
 DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2
 
+class SsmInputs(ct.Structure):
+    """gdn_ssm_inputs (include/gdn_hip.h)."""
+    _fields_ = ([(n, ct.c_void_p) for n in ("x", "dt", "b", "c", "z", "A_log", "D", "dt_bias")] +
+                [(f"{t}_{d}", ct.c_int64) for t in ("x", "dt", "b", "c", "z")
+                 for d in ("batch", "token")] +
+                [(n, ct.c_int) for n in ("batch", "tokens", "heads", "head_dim", "groups",
+                                         "state_dim", "io_dtype", "dt_dtype")] +
+                [("dt_min", ct.c_float), ("dt_max", ct.c_float)])
+
+
+_SSM = ct.POINTER(SsmInputs)
+
 _PROTOS = {
+    "gdn_ssm_step": (hipError_t, [_SSM, vp, fp, i32p, c_int, hipStream_t]),
+    "gdn_ssm_scan_block": (c_int, [_SSM, c_int]),
+    "gdn_ssm_scan_workspace_size": (c_size_t, [_SSM, c_int, c_int, c_int]),
+    "gdn_ssm_scan": (hipError_t, [_SSM, vp, fp, fp, i32p, i32p, c_int, c_int, vp, c_size_t,
+                                  hipStream_t]),
+    "gdn_request_block_rows": (c_int, [c_int] * 3),
+    "gdn_request_blocks": (hipError_t, [i32p, i32p, c_int, c_int, c_int] + [i32p] * 5 +
+                           [hipStream_t]),
+    "gdn_causal_conv1d_prefill": (hipError_t, [vp] * 6 + [c_int] * 5 + [c_int64] * 4 +
+                                  [i32p] + [c_int] * 4 + [hipStream_t]),
+    "gdn_gated_groupnorm_forward": (hipError_t, [vp, c_int64, vp, c_int64, vp, vp, c_int64, c_int,
+                                                 c_int, c_float, c_int, c_int, c_int,
+                                                 hipStream_t]),
+    "gdn_causal_conv1d_update_slots": (hipError_t, [vp] * 5 + [i32p] + [c_int] * 6 +
+                                       [c_int64] * 8 + [c_int] * 3 + [hipStream_t]),
     "deltanet_prefill_workspace_size": (c_size_t, [c_int] * 6),
     "deltanet_tcop_prefill_workspace_size": (c_size_t, [c_int] * 6),
     "deltanet_chunk_prefill": (hipError_t, [vp, vp, vp, fp, fp, vp, fp, fp] + [c_int] * 7 +
