@@ -18,18 +18,20 @@ __device__ __forceinline__ float io_hi(uint32_t u) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16));
 }
 
-// two fp32 values rounded to nearest-even 16-bit values and packed (a low)
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+// two fp32 values rounded to nearest-even 16-bit values and packed (a low): one
+// v_cvt_pk_bf16_f32 / v_cvt_pk_f16_f32.  Not as inline asm: its result may be
+// an MFMA operand and its inputs MFMA results, and the wait states between
+// those and a vector instruction are placed by the compiler, which does not
+// look into asm.
 template <int IO>
 __device__ __forceinline__ uint32_t io_pack(float a, float b) {
-    if constexpr (IO == 0) {
-        uint32_t u;
-        asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(u) : "v"(a), "v"(b));
-        return u;
-    } else {
-        const uint16_t x = __builtin_bit_cast(uint16_t, (_Float16)a);
-        const uint16_t y = __builtin_bit_cast(uint16_t, (_Float16)b);
-        return (uint32_t)x | ((uint32_t)y << 16);
-    }
+    const f32x2 v = {a, b};
+    if constexpr (IO == 0) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, half2v));
 }
 
 template <int IO>
