@@ -295,7 +295,8 @@ hipError_t gdn_causal_conv1d_update(const void* x, void* conv_state, const void*
  *   dt   : [batch][tokens][heads] of dt_dtype (io_dtype or fp32)
  *   A_log: fp32 [heads]; D, dt_bias: fp32 [heads] or null (zeros)
  * A row's heads (groups) lie next to each other; batches and tokens lie
- * *_batch and *_token elements apart (token strides below 2^31).  x, z, b, c
+ * *_batch and *_token elements apart (token strides, and heads x head_dim,
+ * below 2^24).  x, z, b, c
  * are 16-byte aligned with strides that are multiples of 8.  head_dim is a
  * multiple of 16 up to 256, state_dim 16, 32, 64, 128 or 256, 0 <= dt_min <=
  * dt_max.  A token whose inputs are not finite leaves undefined values in its

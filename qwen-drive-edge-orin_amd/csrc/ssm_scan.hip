@@ -33,6 +33,7 @@
 #include "gdn_ssm.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace gdn {
 namespace {
@@ -40,6 +41,8 @@ namespace {
 constexpr int kMaxBlock = 1 << 20;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
+constexpr int kTiles = 2;          // 16-column tiles of a wave
+constexpr int kCols = 16 * kTiles;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Seg {
@@ -57,7 +60,7 @@ struct ScanArgs {
     int segs, seqs, block;
     int slices;          // column slices of a head: ceil(P / PW)
     int tasks;           // slices of a group: heads / groups x slices
-    int quads;           // ceil(tasks / 4): work-groups per group and segment
+    int quads;           // work-groups per group and segment: ceil(tasks / waves)
     f32x4* states;       // [row][group][task] fragments of a slice's state
     float* decays;       // [row][group][task]
 };
@@ -122,12 +125,14 @@ __device__ __forceinline__ s16x8 row_operand(const uint16_t* base, int r, int p)
     return *reinterpret_cast<const s16x8*>(piece_at<PR>(base, r, p));
 }
 
+template <int IO>
 __device__ __forceinline__ f32x4 mma(s16x8 a, s16x8 b, f32x4 c) {
-    return mfma16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
+    if constexpr (IO == 0) return mfma16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
+    else return mfma16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c);
 }
 
-// 8 floats as a sum of bf16 operands: x = t[0] + t[1] (+ t[2])
-template <int TERMS>
+// 8 floats as a sum of 16-bit operands: x = t[0] + t[1] (+ t[2])
+template <int IO, int TERMS>
 __device__ __forceinline__ void split(const float (&x)[8], s16x8 (&t)[TERMS]) {
     float r[8];
 #pragma unroll
@@ -137,72 +142,188 @@ __device__ __forceinline__ void split(const float (&x)[8], s16x8 (&t)[TERMS]) {
         u32x4 w;
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-            w[p] = io_pack<0>(r[2 * p], r[2 * p + 1]);
+            w[p] = io_pack<IO>(r[2 * p], r[2 * p + 1]);
             if (k + 1 < TERMS) {
-                r[2 * p] -= io_lo<0>(w[p]);
-                r[2 * p + 1] -= io_hi<0>(w[p]);
+                r[2 * p] -= io_lo<IO>(w[p]);
+                r[2 * p + 1] -= io_hi<IO>(w[p]);
             }
         }
         t[k] = __builtin_bit_cast(s16x8, w);
     }
 }
 
-// rows [0, n) of a 64-row tile with PR pieces a row, straight into LDS by
-// `waves` waves; rows past n repeat the last one (finite wherever the row is)
-template <int PR>
-__device__ __forceinline__ void stage(const uint16_t* src, int64_t stride, int n, int last_piece,
-                                      uint16_t* lds, int wave, int waves, int lane) {
-    for (int i = wave; i < PR; i += waves) {   // 64 slots of 16 bytes each
-        const int q = 64 * i + lane, r = q / PR, p = (q % PR) ^ swz<PR>(r);
-        const uint16_t* from = src + (int64_t)min(r, n - 1) * stride + 8 * min(p, last_piece);
-        __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void*)(lds + 512 * i),
-                                         16, 0, 0);
-    }
-}
+// A 64-row tile with PR pieces a row on its way into LDS, 64 slots of 16 bytes
+// per load, loads wave, wave + WAVES, ..; rows past n repeat the last one
+// (finite wherever the row is)
+//
+// The load is asm because the compiler, which cannot tell the tiles apart,
+// would wait for it before the next access to any of them, and these are
+// prefetches: who reads a tile waits for vmcnt(0) and a barrier first.  It has
+// no output register, and to the compiler's own waits it is one more
+// operation in flight, which can only make them longer.
+template <int PR, int WAVES>
+struct Stager {
+    static constexpr int kRows = 64 * WAVES / PR;   // rows between a wave's loads
+    const char* base;      // the next chunk's first row
+    uint32_t row;          // bytes from row to row (below 2^25)
+    uint32_t at;           // byte offset of this lane's piece of its first row
+    int last_piece;
+    uint32_t lds;          // byte address of load 0's slots
 
-template <int N, int PT, bool kLocal>
-struct Smem {
-    uint16_t b[64 * N];
-    uint16_t c[kLocal ? 8 : 64 * N];
-    uint16_t x[kWaves][64 * 16 * PT];
-    f32x4 cb[kLocal ? 1 : 10][64];   // (C B^T)^T tiles of the lower triangle, as fragments
-    float c2[kWaves][64], d[kWaves][64], w[kWaves][64];
+    __device__ __forceinline__ int piece(int r, int lane) const { return min((lane % PR) ^ swz<PR>(r), last_piece); }
+
+    __device__ __forceinline__ void init(const uint16_t* src, int64_t stride, int last_piece_,
+                                         const uint16_t* tile, int wave, int lane) {
+        base = reinterpret_cast<const char*>(src);
+        row = 2 * (uint32_t)stride;
+        last_piece = last_piece_;
+        const int r0 = (64 * wave + lane) / PR;
+        at = row * r0 + 16 * piece(r0, lane);
+        lds = __builtin_amdgcn_readfirstlane(
+            (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint16_t*)(tile + 512 * wave));
+    }
+    __device__ __forceinline__ static void send(const char* from, uint32_t off, uint32_t to) {
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                     :: "v"(off), "s"(from), "s"(to) : "memory", "m0");
+    }
+    // the next chunk's n rows, `offset` bytes into the tile
+    __device__ __forceinline__ void load(int n, uint32_t offset, int wave, int lane) {
+        constexpr bool kOneSwizzle = kRows % 16 == 0 || PR <= 4;   // for all rows of a lane
+        if (kOneSwizzle && n == kChunk) {
+            const char* from = base;
+#pragma unroll
+            for (int j = 0; j < PR / WAVES; ++j) {
+                send(from, at, lds + offset + 1024 * WAVES * j);
+                from += kRows * row;
+            }
+        } else {
+            const int r0 = (64 * wave + lane) / PR;
+#pragma unroll
+            for (int j = 0; j < PR / WAVES; ++j) {
+                const int r = r0 + kRows * j;
+                send(base, row * min(r, n - 1) + 16 * piece(r, lane), lds + offset + 1024 * WAVES * j);
+            }
+        }
+        base += kChunk * (uint64_t)row;
+    }
 };
 
-__device__ __forceinline__ int tri(int tt, int st) { return tt * (tt + 1) / 2 + st; }
+// Inclusive sums over lanes 0 .. lane (DPP: within rows of 16, then across)
+__device__ __forceinline__ float lane_prefix(float x) {
+#define GDN_DPP(ctrl, rows)                                                                      \
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(                                  \
+                                       0, __builtin_bit_cast(int, x), ctrl, rows, 0xf, false))
+    GDN_DPP(0x111, 0xf);   // row_shr:1
+    GDN_DPP(0x112, 0xf);
+    GDN_DPP(0x114, 0xf);
+    GDN_DPP(0x118, 0xf);
+    GDN_DPP(0x142, 0xa);   // row_bcast:15 into rows 1 and 3
+    GDN_DPP(0x143, 0xc);   // row_bcast:31 into rows 2 and 3
+#undef GDN_DPP
+    return x;
+}
+
+// The largest of non-negative x over the wave
+__device__ __forceinline__ float wave_max(float x) {
+#define GDN_DPP(ctrl, rows)                                                                       \
+    x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(                           \
+                                               __builtin_bit_cast(int, x),                        \
+                                               __builtin_bit_cast(int, x), ctrl, rows, 0xf, false)))
+    GDN_DPP(0x111, 0xf);
+    GDN_DPP(0x112, 0xf);
+    GDN_DPP(0x114, 0xf);
+    GDN_DPP(0x118, 0xf);
+    GDN_DPP(0x142, 0xa);
+    GDN_DPP(0x143, 0xc);
+#undef GDN_DPP
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+
+// k that brings x >= 0 into [2^14, 2^15), fp16's top binade but one; within
+// +-100, so that 2^k and a few sums of such k stay inside fp32's exponents
+__device__ __forceinline__ int fit_fp16(float x) {
+    const int e = (int)(__builtin_bit_cast(uint32_t, x) >> 23) - 127;
+    return min(max(14 - e, -100), 100);
+}
+
+__device__ __forceinline__ float pow2(int k) {   // -126 <= k <= 127
+    return __builtin_bit_cast(float, (uint32_t)(k + 127) << 23);
+}
+
+template <int N, int PT, int WAVES, bool kLocal>
+struct Smem {
+    uint16_t b[2][64 * N];           // this chunk's and the next one's
+    uint16_t c[kLocal ? 8 : 64 * N];
+    uint16_t x[WAVES][64 * 16 * PT];
+    f32x4 cb[kLocal ? 1 : 10][64];   // (C B^T)^T tiles of the lower triangle, as fragments
+    // per token of the chunk, for each wave's head: c; the step d; the weight
+    // in S; d e^{c_ref - c}, c_ref the last c of the token's 16
+    struct {
+        float c2[64], d[64], w[64], f[64];
+    } tok[WAVES];
+};
+
+__device__ __forceinline__ constexpr int tri(int tt, int st) { return tt * (tt + 1) / 2 + st; }
 
 // kLocal: the first pass (states only)
-template <int IO, int N, int PT, bool kLocal>
-__global__ __launch_bounds__(kThreads) void ssm_scan_kernel(const ScanArgs a) {
+template <int IO, int N, int PT, int WAVES, bool kLocal>
+__global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(const ScanArgs a) {
     constexpr int NT = N / 16, NKB = N / 32, PR = N / 8, XR = 2 * PT, PW = 16 * PT;
-    __shared__ Smem<N, PT, kLocal> sm;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int kParts = IO == 0 ? 3 : 2;   // of w x: 24 or 22 bits
+    __shared__ Smem<N, PT, WAVES, kLocal> sm;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, m = lane & 15;
     const gdn_ssm_inputs& in = a.in;
 
-    // work-groups are dealt round-robin to the XCDs: those of one segment and
-    // group, which share B and C, get ids of one XCD
-    const int total = gridDim.x, per = total / 8, extra = total % 8, xcd = blockIdx.x % 8;
-    const int id = xcd * per + min(xcd, extra) + blockIdx.x / 8;
-    const int quad = id % a.quads, rest = id / a.quads;
-    const int grp = rest % in.groups, row = rest / in.groups;
+    // Work-groups are dealt round-robin to the 8 XCDs.  The quads of a segment
+    // and group, which share B and C, are consecutive on one XCD; the segments
+    // are dealt over all of them, so that short ones even out.
+    const int xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
+    const int quad = nth % a.quads, unit = nth / a.quads * 8 + xcd;
+    const int grp = unit % in.groups, row = unit / in.groups;
     Seg s;
-    if (!segment(a, row, s) || (kLocal && s.last)) return;
-    const int task = quad * kWaves + wave;
+    if (row >= a.rows || !segment(a, row, s) || (kLocal && s.last)) return;
+    const int task = quad * WAVES + wave;
     const bool store = task < a.tasks;   // waves past the group's last slice repeat it
     const int tk = min(task, a.tasks - 1);
     const int h = grp * (in.heads / in.groups) + tk / a.slices;
     const int p0 = (tk % a.slices) * PW;
     const int P = in.head_dim, H = in.heads;
+    auto& tok = sm.tok[wave];
 
     const int bi = a.table ? 0 : s.seq;
     const uint16_t* xp = static_cast<const uint16_t*>(in.x) + bi * in.x_batch + s.t0 * in.x_token + (int64_t)h * P + p0;
     const uint16_t* bp = static_cast<const uint16_t*>(in.b) + bi * in.b_batch + s.t0 * in.b_token + (int64_t)grp * N;
     const uint16_t* cp = static_cast<const uint16_t*>(in.c) + bi * in.c_batch + s.t0 * in.c_token + (int64_t)grp * N;
-    const uint16_t* zp = in.z ? static_cast<const uint16_t*>(in.z) + bi * in.z_batch + s.t0 * in.z_token + (int64_t)h * P + p0 : nullptr;
-    const size_t dp = (size_t)(bi * in.dt_batch + s.t0 * in.dt_token + h);
-    uint16_t* yp = a.y + (((size_t)bi * in.tokens + s.t0) * H + h) * P + p0;
     const int last_piece = (P - p0) / 8 - 1;   // of the head, from p0 on
+    // the chunk's first row of z, y and dt, and byte offsets of this lane's
+    // values from there (row strides are below 2^24)
+    const uint16_t* zp = in.z ? static_cast<const uint16_t*>(in.z) + bi * in.z_batch + s.t0 * in.z_token + (int64_t)h * P + p0 : nullptr;
+    const bool gate = in.z != nullptr;
+    const uint32_t zrow = 2 * (uint32_t)in.z_token, z0 = 16 * min(g, last_piece), zm = m * zrow + z0;
+    const uint32_t yrow = 2 * (uint32_t)(H * P), ym = m * yrow + 16 * g;
+    char* yp = reinterpret_cast<char*>(a.y + ((int64_t)bi * in.tokens + s.t0) * H * P + (int64_t)h * P + p0);
+    const uint32_t dt_size = in.dt_dtype == GDN_DTYPE_FP32 ? 4 : 2, dt_row = (uint32_t)in.dt_token * dt_size;
+    const char* dtp = static_cast<const char*>(in.dt) + (bi * in.dt_batch + s.t0 * in.dt_token + h) * dt_size;
+    auto load_dt = [&](int n) {   // of the next chunk's token `lane`, or of its last
+        const char* at = dtp + (uint32_t)min(lane, n - 1) * dt_row;
+        dtp += kChunk * (uint64_t)dt_row;
+        return dt_size == 4 ? *reinterpret_cast<const float*>(at) : io_elem<IO>(at, 0);
+    };
+    Stager<PR, WAVES> bst, cst;
+    Stager<XR, 1> xst;
+    bst.init(bp, in.b_token, PR, sm.b[0], wave, lane);
+    if (!kLocal) cst.init(cp, in.c_token, PR, sm.c, wave, lane);
+    xst.init(xp, in.x_token, last_piece, sm.x[wave], 0, lane);
+    float raw_dt = 0.f;
+    if (s.n > 0) {
+        const int n = min(s.n, kChunk);
+        raw_dt = load_dt(n);
+        bst.load(n, 0, wave, lane);
+        if (!kLocal) cst.load(n, 0, wave, lane);
+        xst.load(n, 0, 0, lane);
+    }
 
     // state tiles [nt][pt]: lane (g, m), element i is
     // n = 32 (nt / 2) + 8 g + 4 (nt % 2) + i, p = p0 + perm(pt, m)
@@ -213,18 +334,22 @@ __global__ __launch_bounds__(kThreads) void ssm_scan_kernel(const ScanArgs a) {
         for (int pt = 0; pt < PT; ++pt) S[nt][pt] = zero4();
     const size_t hs = ((size_t)s.seq * H + h) * N * P;
     const size_t rec = ((size_t)row * in.groups + grp) * a.tasks + tk;   // state record
-    auto n_of = [&](int nt, int i) { return 32 * (nt >> 1) + 8 * g + 4 * (nt & 1) + i; };
-    auto p_of = [&](int pt) { return p0 + 32 * (pt >> 1) + 8 * (m >> 2) + 4 * (pt & 1) + (m & 3); };
+    // element (nt, pt, i) of a lane in a state [N][P]: so + n_off(nt, i) P + p_off(pt)
+    const size_t so = hs + (size_t)(8 * g) * P + p0 + 8 * (m >> 2) + (m & 3);
+    auto n_off = [](int nt, int i) { return 32 * (nt >> 1) + 4 * (nt & 1) + i; };
+    auto p_off = [](int pt) { return 32 * (pt >> 1) + 4 * (pt & 1); };
+    const int p_lane = p0 + 8 * (m >> 2) + (m & 3);
     if (s.idx == 0) {
         if (a.s0) {
+            const float* from = a.s0 + so;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int pt = 0; pt < PT; ++pt)
+                if (p_lane + p_off(pt) < P) {
 #pragma unroll
-                for (int pt = 0; pt < PT; ++pt)
-                    if (p_of(pt) < P) {
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) S[nt][pt][i] = a.s0[hs + (size_t)n_of(nt, i) * P + p_of(pt)];
-                    }
+                        for (int i = 0; i < 4; ++i) S[nt][pt][i] = from[n_off(nt, i) * P + p_off(pt)];
+                }
         }
     } else if (!kLocal) {
         const f32x4* from = a.states + (rec - (size_t)in.groups * a.tasks) * (NT * PT * 64) + lane;
@@ -238,52 +363,92 @@ __global__ __launch_bounds__(kThreads) void ssm_scan_kernel(const ScanArgs a) {
     const float bias = in.dt_bias ? in.dt_bias[h] : 0.f;
     const float D = in.D ? in.D[h] : 0.f;
     float log_total = 0.f;   // the segment's base-2 log decay
-    float* const c2s = sm.c2[wave];
-    float* const dss = sm.d[wave];
-    float* const wss = sm.w[wave];
-    const uint16_t* const xs = sm.x[wave];
 
-    for (int t0 = 0; t0 < s.n; t0 += kChunk) {
-        const int n = min(s.n - t0, kChunk);
-        __syncthreads();   // the previous chunk's tiles are read
-        stage<PR>(bp + t0 * in.b_token, in.b_token, n, PR, sm.b, wave, kWaves, lane);
-        if (!kLocal) stage<PR>(cp + t0 * in.c_token, in.c_token, n, PR, sm.c, wave, kWaves, lane);
-        stage<XR>(xp + t0 * in.x_token, in.x_token, n, last_piece, sm.x[wave], 0, 1, lane);
+    // fp16: what enters an MFMA is scaled by a power of two first, so that
+    // neither large nor small values leave the five exponent bits.  The
+    // accumulators S hold 2^kappa times the state.
+    int kappa = 0;
+    float d_max = 0.f, w_max = 0.f;
 
-        // token `lane`: step, log decay, its sums from the chunk's start and end
-        const size_t di = dp + (size_t)(t0 + min(lane, n - 1)) * in.dt_token;
-        const float raw = in.dt_dtype == GDN_DTYPE_FP32 ? io_elem<2>(in.dt, di) : io_elem<IO>(in.dt, di);
-        const float dv = lane < n ? ssm_delta(raw, bias, in.dt_min, in.dt_max) : 0.f;
-        const float l2 = fmaxf(A2 * dv, -150.f);
-        float up = l2, down = l2;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const float u = __shfl_up(up, off, 64), v = __shfl_down(down, off, 64);
-            if (lane >= off) up += u;
-            if (lane + off < 64) down += v;
+    // Token `lane` of a chunk of n: step, log decay, its sums from the chunk's
+    // start and from its end
+    auto token_vectors = [&](float raw, int n) {
+        const float d = lane < n ? ssm_delta(raw, bias, in.dt_min, in.dt_max) : 0.f;
+        const float l2 = fmaxf(A2 * d, -150.f);
+        const float c2 = lane_prefix(l2);
+        // lane i of the reversed order is token 63 - i
+        const float back = lane_prefix(__shfl(l2, 63 - lane, 64));
+        const float after = __shfl(back, 62 - lane, 64);   // tokens lane + 1 ..
+        tok.c2[lane] = c2;
+        tok.d[lane] = d;
+        const float w = d * __builtin_amdgcn_exp2f(lane < 63 ? after : 0.f);
+        tok.w[lane] = w;
+        if (IO == 1) {
+            d_max = wave_max(d);
+            w_max = wave_max(w);
         }
-        const float after = __shfl_down(down, 1, 64);
-        c2s[lane] = up;
-        dss[lane] = dv;
-        wss[lane] = dv * __builtin_amdgcn_exp2f(lane < 63 ? after : 0.f);
-        const float total2 = __shfl(up, 63, 64);
-        log_total += total2;
-        __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the tiles are in LDS
-        __syncthreads();
+        if (!kLocal) tok.f[lane] = d * __builtin_amdgcn_exp2f(__shfl(c2, lane | 15, 64) - c2);
+    };
 
-        if constexpr (!kLocal) {
-            // (C B^T)^T: rows s of tile st, columns t of tile tt
-            for (int k = wave; k < 10; k += kWaves) {
-                const int tt = k < 1 ? 0 : k < 3 ? 1 : k < 6 ? 2 : 3, st = k - tt * (tt + 1) / 2;
-                f32x4 acc = zero4();
+    f32x4 Dd;   // D on the diagonal of a tile
 #pragma unroll
-                for (int kb = 0; kb < NKB; ++kb)
-                    acc = mma(row_operand<PR>(sm.b, 16 * st + m, 4 * kb + g),
-                              row_operand<PR>(sm.c, 16 * tt + m, 4 * kb + g), acc);
-                sm.cb[k][lane] = acc;
+    for (int i = 0; i < 4; ++i) Dd[i] = 4 * g + i == m ? D : 0.f;
+    const bool cols[2] = {store && g <= last_piece, store && 4 + g <= last_piece};
+
+    int cur = 0;
+    for (int t0 = 0; t0 < s.n; t0 += kChunk, cur ^= 1) {
+        const int n = min(s.n - t0, kChunk);
+        const uint16_t* const bs = sm.b[cur];
+        const uint16_t* const cs_ = sm.c;
+        const uint16_t* const xs = sm.x[wave];
+
+        __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this wave's part of the tiles is in LDS
+        __syncthreads();                      // and the others'; the last chunk's tiles are read
+        const float raw = raw_dt;
+        const int next = min(s.n - t0 - kChunk, kChunk);   // tokens of the next chunk
+        if (next > 0) {
+            raw_dt = load_dt(next);
+            bst.load(next, (cur ^ 1) * (uint32_t)sizeof(sm.b[0]), wave, lane);
+        }
+        u32x4 zr[PT / 2][4];
+        f32x4 Y[PT][4];
+        if constexpr (!kLocal) {
+            if (gate) {
+                const char* z = reinterpret_cast<const char*>(zp);
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt) {
+                    // (rows past the chunk: its first row again)
+                    const uint32_t off = 16 * tt + m < n ? zm + 16 * tt * zrow : z0;
+#pragma unroll
+                    for (int q = 0; q < PT / 2; ++q)
+                        zr[q][tt] = *reinterpret_cast<const u32x4*>(z + (4 * q + g <= last_piece ? off + 64 * q : off));
+                }
+                zp += kChunk * (int64_t)in.z_token;
             }
-            // S^T C^T: rows p, columns t
-            f32x4 Y[PT][4];
+        }
+        // From here to the barrier there is no branch: the token vectors' chain
+        // of lane exchanges and C B^T's of LDS reads run beside S^T C^T
+        token_vectors(raw, n);
+        float s_max = 0.f;
+        int k_s = 0;
+        if constexpr (IO == 1) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int pt = 0; pt < PT; ++pt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s_max = fmaxf(s_max, fabsf(S[nt][pt][i]));
+            s_max = wave_max(s_max);
+        }
+        if constexpr (!kLocal) {
+            // (C B^T)^T: rows s, columns t of tile `wave` (of the tiles above the
+            // diagonal, which nobody reads, too); S^T C^T: rows p, columns t
+            static_assert(WAVES == 4, "a column tile of C B^T per wave");
+            if constexpr (IO == 1) k_s = fit_fp16(s_max);
+            const float s_scale = IO == 1 ? pow2(k_s) : 1.f;
+            f32x4 acc[4];
+#pragma unroll
+            for (int st = 0; st < 4; ++st) acc[st] = zero4();
 #pragma unroll
             for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
@@ -292,7 +457,11 @@ __global__ __launch_bounds__(kThreads) void ssm_scan_kernel(const ScanArgs a) {
             for (int kb = 0; kb < NKB; ++kb) {
                 s16x8 cop[4];
 #pragma unroll
-                for (int tt = 0; tt < 4; ++tt) cop[tt] = row_operand<PR>(sm.c, 16 * tt + m, 4 * kb + g);
+                for (int tt = 0; tt < 4; ++tt) cop[tt] = row_operand<PR>(cs_, 16 * tt + m, 4 * kb + g);
+                const s16x8 own = row_operand<PR>(cs_, 16 * wave + m, 4 * kb + g);
+#pragma unroll
+                for (int st = 0; st < 4; ++st)
+                    acc[st] = mma<IO>(row_operand<PR>(bs, 16 * st + m, 4 * kb + g), own, acc[st]);
 #pragma unroll
                 for (int pt = 0; pt < PT; ++pt) {
                     float v[8];
@@ -300,40 +469,73 @@ __global__ __launch_bounds__(kThreads) void ssm_scan_kernel(const ScanArgs a) {
                     for (int i = 0; i < 4; ++i) {
                         v[i] = S[2 * kb][pt][i];
                         v[4 + i] = S[2 * kb + 1][pt][i];
+                        if (IO == 1) {
+                            v[i] *= s_scale;
+                            v[4 + i] *= s_scale;
+                        }
                     }
                     s16x8 sop[2];
-                    split<2>(v, sop);
+                    split<IO, 2>(v, sop);
 #pragma unroll
-                    for (int tt = 0; tt < 4; ++tt) {
-                        Y[pt][tt] = mma(sop[0], cop[tt], Y[pt][tt]);
-                        Y[pt][tt] = mma(sop[1], cop[tt], Y[pt][tt]);
-                    }
+                    for (int k = 1; k >= 0; --k)
+#pragma unroll
+                        for (int tt = 0; tt < 4; ++tt) Y[pt][tt] = mma<IO>(sop[k], cop[tt], Y[pt][tt]);
                 }
+            }
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+                if (st <= wave) sm.cb[tri(wave, st)][lane] = acc[st];
+        }
+        s16x8 xop[PT][2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int pt = 0; pt < PT; ++pt) xop[pt][kb] = tr_operand<XR>(xs, pt, kb, lane);
+        __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): x is read
+        __syncthreads();   // the vectors and C B^T are complete, C is read
+        if (next > 0) {
+            // (z is here before they go out: waits count operations in order)
+            if (!kLocal && gate) {
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+                    for (int q = 0; q < PT / 2; ++q) asm volatile("" ::"v"(zr[q][tt]));
+            }
+            if (!kLocal) cst.load(next, 0, wave, lane);
+            xst.load(next, 0, 0, lane);
+        }
+
+        if constexpr (!kLocal) {
+            // fp16: M, at most max |C B^T| max d + |D|, times 2^k_m, and Y with it
+            int k_m = 0;
+            f32x4 Dm = Dd;
+            if constexpr (IO == 1) {
+                float top = 0.f;
+#pragma unroll
+                for (int k = 0; k < 10; ++k) {
+                    const f32x4 cb = sm.cb[k][lane];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(cb[i]));
+                }
+                k_m = fit_fp16(2.f * fmaxf(wave_max(top) * d_max, fabsf(D)));
+                Dm *= pow2(k_m);
             }
             float ct[4];
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt) {
-                ct[tt] = c2s[16 * tt + m];
-                const float e = __builtin_amdgcn_exp2f(ct[tt]);
+                ct[tt] = tok.c2[16 * tt + m];
+                const float e = __builtin_amdgcn_exp2f(IO == 1 ? ct[tt] + (float)(k_m - k_s - kappa) : ct[tt]);
+                if (IO == 1) ct[tt] += (float)k_m;
 #pragma unroll
                 for (int pt = 0; pt < PT; ++pt) Y[pt][tt] *= e;
             }
-            __syncthreads();   // C B^T is complete
-
-            // + X^T M^T, M[t][s] = (C B^T) e^{c_t - c_s} d_s for s <= t
+            // + X^T M^T, M[t][s] = (C B^T) e^{c_t - c_s} d_s for s <= t, + D for s = t.
+            // Below the diagonal tiles the exponential is a product of one per
+            // column and one per row, both at most 1.
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                s16x8 xop[PT];
+            for (int tt = 0; tt < 4; ++tt) {
 #pragma unroll
-                for (int pt = 0; pt < PT; ++pt) xop[pt] = tr_operand<XR>(xs, pt, kb, lane);
-                f32x4 cs[2], ds[2];
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    cs[q] = *reinterpret_cast<const f32x4*>(c2s + 32 * kb + 16 * q + 4 * g);
-                    ds[q] = *reinterpret_cast<const f32x4*>(dss + 32 * kb + 16 * q + 4 * g);
-                }
-#pragma unroll
-                for (int tt = 2 * kb; tt < 4; ++tt) {
+                for (int kb = 0; kb <= tt / 2; ++kb) {
                     float v[8];
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
@@ -341,86 +543,131 @@ __global__ __launch_bounds__(kThreads) void ssm_scan_kernel(const ScanArgs a) {
                         if (st > tt) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) v[4 * q + i] = 0.f;
-                            continue;
-                        }
-                        const f32x4 cb = sm.cb[tri(tt, st)][lane];
+                        } else if (st == tt) {
+                            const f32x4 cb = sm.cb[tri(tt, st)][lane];
+                            const f32x4 cs = *reinterpret_cast<const f32x4*>(tok.c2 + 16 * st + 4 * g);
+                            const f32x4 ds = *reinterpret_cast<const f32x4*>(tok.d + 16 * st + 4 * g);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float e = cb[i] * __builtin_amdgcn_exp2f(ct[tt] - cs[q][i]) * ds[q][i];
-                            v[4 * q + i] = st < tt || 4 * g + i <= m ? e : 0.f;
+                            for (int i = 0; i < 4; ++i) {
+                                const float e = cb[i] * __builtin_amdgcn_exp2f(ct[tt] - cs[i]) * ds[i];
+                                v[4 * q + i] = (4 * g + i <= m ? e : 0.f) + Dm[i];
+                            }
+                        } else {
+                            const f32x4 cb = sm.cb[tri(tt, st)][lane];
+                            const f32x4 fs = *reinterpret_cast<const f32x4*>(tok.f + 16 * st + 4 * g);
+                            const float ht = __builtin_amdgcn_exp2f(ct[tt] - tok.c2[16 * st + 15]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[4 * q + i] = cb[i] * (fs[i] * ht);
                         }
                     }
                     s16x8 mop[2];
-                    split<2>(v, mop);
+                    split<IO, 2>(v, mop);
 #pragma unroll
-                    for (int pt = 0; pt < PT; ++pt) {
-                        Y[pt][tt] = mma(xop[pt], mop[0], Y[pt][tt]);
-                        Y[pt][tt] = mma(xop[pt], mop[1], Y[pt][tt]);
-                    }
+                    for (int k = 1; k >= 0; --k)
+#pragma unroll
+                        for (int pt = 0; pt < PT; ++pt) Y[pt][tt] = mma<IO>(xop[pt][kb], mop[k], Y[pt][tt]);
                 }
             }
-            // + D x, the gate, out: 8 channels of one token a lane
+            // the gate, out: 8 channels of one token a lane
+            if constexpr (IO == 1) {
+                const float down = pow2(-k_m);
+#pragma unroll
+                for (int pt = 0; pt < PT; ++pt)
+#pragma unroll
+                    for (int tt = 0; tt < 4; ++tt) Y[pt][tt] *= down;
+            }
+            if (gate) {
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+                    for (int q = 0; q < PT / 2; ++q)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            f32x4& yv = Y[2 * q + (k >> 1)][tt];
+                            yv[2 * (k & 1)] *= silu_fast(io_lo<IO>(zr[q][tt][k]));
+                            yv[2 * (k & 1) + 1] *= silu_fast(io_hi<IO>(zr[q][tt][k]));
+                        }
+            }
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt) {
-                const int t = 16 * tt + m;
 #pragma unroll
                 for (int q = 0; q < PT / 2; ++q) {
-                    const int p = 32 * q + 8 * g;   // from p0
-                    if (!store || t >= n || p0 + p >= P) continue;
-                    const u32x4 xr = __builtin_bit_cast(u32x4, row_operand<XR>(xs, t, 4 * q + g));
-                    u32x4 zr = {0, 0, 0, 0};
-                    if (zp) zr = *reinterpret_cast<const u32x4*>(zp + (int64_t)(t0 + t) * in.z_token + p);
-                    u32x4 o;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const f32x4& yv = Y[2 * q + (k >> 1)][tt];
-                        float u = yv[2 * (k & 1)] + D * io_lo<IO>(xr[k]);
-                        float v = yv[2 * (k & 1) + 1] + D * io_hi<IO>(xr[k]);
-                        if (zp) {
-                            u *= silu_fast(io_lo<IO>(zr[k]));
-                            v *= silu_fast(io_hi<IO>(zr[k]));
-                        }
-                        o[k] = io_pack<IO>(u, v);
-                    }
-                    *reinterpret_cast<u32x4*>(yp + (size_t)(t0 + t) * H * P + p) = o;
+                    const f32x4 &u = Y[2 * q][tt], &v = Y[2 * q + 1][tt];
+                    const u32x4 o = {io_pack<IO>(u[0], u[1]), io_pack<IO>(u[2], u[3]),
+                                     io_pack<IO>(v[0], v[1]), io_pack<IO>(v[2], v[3])};
+                    if (cols[q] && 16 * tt + m < n) *reinterpret_cast<u32x4*>(yp + (ym + 16 * tt * yrow + 64 * q)) = o;
                 }
             }
+            yp += kChunk * (uint64_t)yrow;
         }
 
         // S <- e^{c_Q} S + B^T (w x)
-        const float dec = __builtin_amdgcn_exp2f(total2);
+        const float total2 = tok.c2[63];
+        float dec = __builtin_amdgcn_exp2f(total2), w_scale = 1.f;
+        log_total += total2;
+        if constexpr (IO == 1) {
+            // the new kappa: the larger of the decayed state and w x fits
+            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+            u16x2 top = {0, 0};
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int pt = 0; pt < PT; ++pt)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        top = __builtin_elementwise_max(
+                            top, __builtin_bit_cast(u16x2, __builtin_bit_cast(u32x4, xop[pt][kb])[k] & 0x7fff7fffu));
+            const uint16_t xm = top[0] > top[1] ? top[0] : top[1];
+            const float wx_max = wave_max(fabsf((float)__builtin_bit_cast(_Float16, xm))) * w_max;
+            const int next_kappa = fit_fp16(fmaxf(dec * s_max * pow2(-kappa), wx_max));
+            // (their difference may pass 2^127 where the state is 0 or decays to nothing)
+            dec = dec * s_max == 0.f ? 0.f : dec * pow2(min(next_kappa - kappa, 127));
+            kappa = next_kappa;
+            w_scale = pow2(kappa);
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int pt = 0; pt < PT; ++pt) S[nt][pt] *= dec;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-            s16x8 wx[PT][3];
-            const f32x4 w0 = *reinterpret_cast<const f32x4*>(wss + 32 * kb + 4 * g);
-            const f32x4 w1 = *reinterpret_cast<const f32x4*>(wss + 32 * kb + 16 + 4 * g);
+            s16x8 wx[PT][kParts];
+            const f32x4 w0 = *reinterpret_cast<const f32x4*>(tok.w + 32 * kb + 4 * g);
+            const f32x4 w1 = *reinterpret_cast<const f32x4*>(tok.w + 32 * kb + 16 + 4 * g);
 #pragma unroll
             for (int pt = 0; pt < PT; ++pt) {
-                const u32x4 xr = __builtin_bit_cast(u32x4, tr_operand<XR>(xs, pt, kb, lane));
+                const u32x4 xr = __builtin_bit_cast(u32x4, xop[pt][kb]);
                 float v[8];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const f32x4& w = k < 2 ? w0 : w1;
                     v[2 * k] = io_lo<IO>(xr[k]) * w[2 * (k & 1)];
                     v[2 * k + 1] = io_hi<IO>(xr[k]) * w[2 * (k & 1) + 1];
+                    if (IO == 1) {
+                        v[2 * k] *= w_scale;
+                        v[2 * k + 1] *= w_scale;
+                    }
                 }
-                split<3>(v, wx[pt]);
+                split<IO, kParts>(v, wx[pt]);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const s16x8 bop = tr_operand<PR>(sm.b, nt, kb, lane);
+                const s16x8 bop = tr_operand<PR>(bs, nt, kb, lane);
 #pragma unroll
-                for (int k = 2; k >= 0; --k)   // the smallest parts first
+                for (int k = kParts - 1; k >= 0; --k)   // the smallest parts first
 #pragma unroll
-                    for (int pt = 0; pt < PT; ++pt) S[nt][pt] = mma(bop, wx[pt][k], S[nt][pt]);
+                    for (int pt = 0; pt < PT; ++pt) S[nt][pt] = mma<IO>(bop, wx[pt][k], S[nt][pt]);
             }
         }
     }
 
+    if constexpr (IO == 1) {
+        const float down = pow2(-kappa);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int pt = 0; pt < PT; ++pt) S[nt][pt] *= down;
+    }
     if (!store) return;
     if (kLocal) {
         f32x4* to = a.states + rec * (NT * PT * 64) + lane;
@@ -430,34 +677,69 @@ __global__ __launch_bounds__(kThreads) void ssm_scan_kernel(const ScanArgs a) {
             for (int pt = 0; pt < PT; ++pt) to[(nt * PT + pt) * 64] = S[nt][pt];
         if (lane == 0) a.decays[rec] = __builtin_amdgcn_exp2f(log_total);
     } else if (s.last) {
+        float* to = a.sf + so;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int pt = 0; pt < PT; ++pt)
+            if (p_lane + p_off(pt) < P) {
 #pragma unroll
-            for (int pt = 0; pt < PT; ++pt)
-                if (p_of(pt) < P) {
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) a.sf[hs + (size_t)n_of(nt, i) * P + p_of(pt)] = S[nt][pt][i];
-                }
+                    for (int i = 0; i < 4; ++i) to[n_off(nt, i) * P + p_off(pt)] = S[nt][pt][i];
+            }
     }
 }
 
 // The states behind segments 1, 2, .. of a sequence from its segments' own:
-// R_j = decay_j R_{j-1} + L_j in place, elementwise (fragment order)
+// R_j = decay_j R_{j-1} + L_j in place, elementwise (fragment order), kAhead
+// segments' loads ahead of the products, so that the chain waits for memory
+// once per kAhead segments.  V is f32x4, or float where that leaves too few
+// threads to carry the traffic (launch_scan).
+template <typename V>
 __global__ __launch_bounds__(kThreads) void ssm_join_kernel(const ScanArgs a, int elems, int parts) {
-    const int id = blockIdx.x;
-    const int part = id % parts, task = id / parts % (a.in.groups * a.tasks), row0 = id / parts / (a.in.groups * a.tasks);
-    int row = a.table ? row0 : row0 * a.segs;
-    Seg s;
-    if (!segment(a, row, s) || s.idx != 0 || s.last) return;
+    const int64_t all = (int64_t)a.in.groups * a.tasks;   // records of a segment
+    const int part = blockIdx.x % parts, rest = blockIdx.x / parts;
+    const int rec = rest % (int)all, seq = rest / (int)all;
+    int row = seq * a.segs, count = a.segs;   // the sequence's first segment, and how many
+    if (a.table) {
+        int lo = 0, hi = a.rows;   // (-1 behind the last block is past every sequence)
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if ((unsigned)a.table[mid].x >= (unsigned)seq) hi = mid;
+            else lo = mid + 1;
+        }
+        row = lo;
+        if (row >= a.rows || a.table[row].x != seq) return;
+        for (int base = row;; base += 64) {
+            const int r = base + (threadIdx.x & 63);
+            const unsigned long long other = __ballot(r >= a.rows || a.table[min(r, a.rows - 1)].x != seq);
+            if (other != 0) {
+                count = base - row + __builtin_ctzll(other);
+                break;
+            }
+        }
+    }
     const int e = part * kThreads + threadIdx.x;
-    if (e >= elems) return;
-    const size_t all = (size_t)a.in.groups * a.tasks;
-    f32x4 R = a.states[((size_t)row * all + task) * elems + e];
-    const int seq = s.seq;
-    while (++row < a.rows && segment(a, row, s) && s.seq == seq && !s.last) {
-        f32x4* at = a.states + ((size_t)row * all + task) * elems + e;
-        R = R * a.decays[(size_t)row * all + task] + *at;
-        *at = R;
+    if (count < 3 || e >= elems) return;
+    V* const at = reinterpret_cast<V*>(a.states) + (row * all + rec) * elems + e;
+    const float* const decay = a.decays + row * all + rec;
+    const int64_t step = all * elems;
+    constexpr int kAhead = 8;
+    V R = at[0];
+    for (int j0 = 1; j0 < count - 1; j0 += kAhead) {
+        V L[kAhead];
+        float d[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const bool on = j0 + k < count - 1;
+            L[k] = on ? at[(j0 + k) * step] : V{};
+            d[k] = on ? decay[(j0 + k) * all] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (j0 + k < count - 1) {
+                R = R * d[k] + L[k];
+                at[(j0 + k) * step] = R;
+            }
     }
 }
 
@@ -547,10 +829,8 @@ bool scan_sizes_ok(const gdn_ssm_inputs* in, int seqs, int block, bool packed) {
 
 // Whether the chunked scan has an instance; the rest takes the recurrence
 bool chunked(const gdn_ssm_inputs* in) {
-    return in->io_dtype == GDN_DTYPE_BF16 && in->state_dim >= 64;
+    return in->state_dim >= 64;
 }
-
-int cols_of(const gdn_ssm_inputs* in) { return in->state_dim == 256 ? 32 : 64; }
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
@@ -563,8 +843,7 @@ struct Layout {
     Layout(const gdn_ssm_inputs* in, int seqs, int block, bool packed) {
         segs = packed ? 0 : std::max(1, (in->tokens + block - 1) / block);
         rows = packed ? (int64_t)in->tokens / block + seqs : (int64_t)segs * seqs;
-        const int pw = cols_of(in);
-        slices = (in->head_dim + pw - 1) / pw;
+        slices = (in->head_dim + kCols - 1) / kCols;
         tasks = in->heads / in->groups * slices;
         quads = (tasks + kWaves - 1) / kWaves;
         size_t off = 0;
@@ -575,31 +854,36 @@ struct Layout {
         // no states where every sequence is one segment
         const size_t recs = packed || segs > 1 ? (size_t)rows * in->groups * tasks : 0;
         states = off;
-        off += align256(recs * in->state_dim * pw * 4);
+        off += align256(recs * in->state_dim * kCols * 4);
         decays = off;
         off += align256(recs * 4);
         total = std::max<size_t>(off, 256);
     }
 };
 
-template <int IO, int N, int PT>
+template <int IO, int N, int PT, int WAVES>
 hipError_t launch_scan(const ScanArgs& a, hipStream_t stream) {
-    const int64_t groups = (int64_t)a.rows * a.in.groups * a.quads;
+    const int64_t groups = ((int64_t)a.rows * a.in.groups + 7) / 8 * 8 * a.quads;
     if (groups > 0x7fffffff) return hipErrorInvalidValue;
     if (a.table || a.segs > 1) {
-        hipLaunchKernelGGL((ssm_scan_kernel<IO, N, PT, true>), dim3((unsigned)groups),
-                           dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL((ssm_scan_kernel<IO, N, PT, WAVES, true>), dim3((unsigned)groups),
+                           dim3(64 * WAVES), 0, stream, a);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         if (a.table || a.segs > 2) {
-            const int elems = N * PT * 4, parts = (elems + kThreads - 1) / kThreads;
-            const int64_t join = (int64_t)(a.table ? a.rows : a.seqs) * a.in.groups * a.tasks * parts;
-            if (join > 0x7fffffff) return hipErrorInvalidValue;
-            hipLaunchKernelGGL(ssm_join_kernel, dim3((unsigned)join), dim3(kThreads), 0, stream, a,
-                               elems, parts);
+            // 16 bytes a thread from 2^17 such threads on (8 sequences of 2..7
+            // segments x 128 records: 13 us against 35 with 4 bytes; one of 64
+            // segments x 32 records: 30 us against 15)
+            const int64_t records = (int64_t)a.seqs * a.in.groups * a.tasks;
+            const bool wide = records * N * PT * 4 >= 1 << 17;
+            const int elems = N * PT * (wide ? 4 : 16), parts = (elems + kThreads - 1) / kThreads;
+            if (records * parts > 0x7fffffff) return hipErrorInvalidValue;
+            const dim3 grid((unsigned)(records * parts));
+            if (wide) hipLaunchKernelGGL(ssm_join_kernel<f32x4>, grid, dim3(kThreads), 0, stream, a, elems, parts);
+            else hipLaunchKernelGGL(ssm_join_kernel<float>, grid, dim3(kThreads), 0, stream, a, elems, parts);
             if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         }
     }
-    hipLaunchKernelGGL((ssm_scan_kernel<IO, N, PT, false>), dim3((unsigned)groups), dim3(kThreads), 0,
+    hipLaunchKernelGGL((ssm_scan_kernel<IO, N, PT, WAVES, false>), dim3((unsigned)groups), dim3(64 * WAVES), 0,
                        stream, a);
     return hipGetLastError();
 }
@@ -607,9 +891,9 @@ hipError_t launch_scan(const ScanArgs& a, hipStream_t stream) {
 template <int IO>
 hipError_t launch_any(const ScanArgs& a, hipStream_t stream) {
     switch (a.in.state_dim) {
-        case 64: return launch_scan<IO, 64, 4>(a, stream);
-        case 128: return launch_scan<IO, 128, 4>(a, stream);
-        default: return launch_scan<IO, 256, 2>(a, stream);
+        case 64: return launch_scan<IO, 64, kTiles, kWaves>(a, stream);
+        case 128: return launch_scan<IO, 128, kTiles, kWaves>(a, stream);
+        default: return launch_scan<IO, 256, kTiles, kWaves>(a, stream);
     }
 }
 
@@ -634,15 +918,56 @@ hipError_t form_table(const int32_t* cu, int seqs, int total, int block, int row
 
 using namespace gdn;
 
+// Microseconds of `groups` work-groups of `chunks` chunks each on 256 CUs that
+// hold `deep` of them at a time: a chunk takes t[k - 1] with k on a CU, and a
+// group `start` on top.
+static double passes_us(double groups, double chunks, int deep, const double* t, double start) {
+    const double full = std::floor(groups / (256.0 * deep));
+    const double rest = groups - full * 256 * deep;
+    double us = full * (chunks * t[deep - 1] + start);
+    if (rest > 0) us += chunks * t[std::min(deep, (int)std::ceil(rest / 256)) - 1] + start;
+    return us;
+}
+
+// The run of chunks with the least estimated time.  Longer runs leave CUs idle
+// or the last round of work-groups thin, shorter ones move more states (16 KB
+// to 64 KB a record and pass).  The constants are measured at state_dim 128
+// (main pass: 5.7 and 8.8 us a chunk with one and two groups on a CU; first pass
+// 2.9, 3.3 and 3.6 with one to three; about 5 us to start a group from its
+// state), the rule's choices at most 16 % slower than the best of 1 .. 256
+// chunks over 19 calls (77 to 65,536 tokens, 8 to 128 heads, 1 to 101 sequences),
+// 3 % on average.
 extern "C" int gdn_ssm_scan_block(const gdn_ssm_inputs* in, int num_seqs) {
     if (!ssm_sizes_ok(in) || num_seqs < 1 || in->tokens > (1 << 30)) return 0;
-    // about two waves per SIMD of a 256-CU chip
-    const int pw = cols_of(in);
-    const int64_t slices = (int64_t)in->heads * ((in->head_dim + pw - 1) / pw);
-    const int64_t tokens = (int64_t)in->batch * in->tokens;
-    const int64_t want = std::max<int64_t>(1, 2048 / slices);
-    const int64_t block = (tokens + want * kChunk - 1) / (want * kChunk) * kChunk;
-    return (int)std::min<int64_t>(std::max<int64_t>(block, kChunk), kMaxBlock);
+    const int tasks = in->heads / in->groups * ((in->head_dim + kCols - 1) / kCols);
+    const double units = (double)in->groups * ((tasks + kWaves - 1) / kWaves);
+    const bool packed = in->batch == 1 && num_seqs > 1;
+    // chunks of a sequence (of the average one, half a chunk of it partial)
+    const double tokens = packed ? (double)in->tokens / num_seqs : in->tokens;
+    const double per_seq = std::max(1.0, packed ? tokens / kChunk + 0.5 : std::ceil(tokens / kChunk));
+    // a group's chunks: packed sequences differ, the longest of a few is about
+    // 1.7 times the average
+    const double longest = packed ? 1.7 * per_seq : per_seq;
+    const double main_t[2] = {5.7, 8.8}, local_t[3] = {2.9, 3.3, 3.6};
+    const double record_us = (double)in->groups * tasks * in->state_dim * kCols * 4 / 5e6;
+    const double scale = in->state_dim / 128.0;
+    const int deep = in->state_dim == 256 ? 1 : 2, local_deep = in->state_dim == 256 ? 1 : 3;
+    int best = 1;
+    double least = 0;
+    for (int c = 1; c <= kMaxBlock / kChunk; c += c < 16 ? 1 : c / 8) {
+        const double segs = packed ? std::max(1.0, per_seq / c + 0.5) : std::ceil(per_seq / c);
+        double us = passes_us(num_seqs * segs * units, std::min<double>(c, longest), deep, main_t, 5) * scale;
+        if (segs > 1)
+            us += 3 + passes_us(num_seqs * (segs - 1) * units, std::min<double>(c, longest), local_deep, local_t,
+                                4) * scale;
+        if (segs > 2) us += 4 + 2 * num_seqs * (segs - 2) * record_us;
+        if (c == 1 || us < least) {
+            least = us;
+            best = c;
+        }
+        if (c >= (packed ? 4 : 1) * per_seq) break;
+    }
+    return best * kChunk;
 }
 
 extern "C" size_t gdn_ssm_scan_workspace_size(const gdn_ssm_inputs* in, int num_seqs, int block,
@@ -692,5 +1017,5 @@ extern "C" hipError_t gdn_ssm_scan(const gdn_ssm_inputs* in, void* y, const floa
             a.table = table;
         }
     }
-    return launch_any<0>(a, stream);
+    return in->io_dtype == GDN_DTYPE_BF16 ? launch_any<0>(a, stream) : launch_any<1>(a, stream);
 }

@@ -33,6 +33,8 @@ int io_dtype(const at::Tensor& x) {
     return x.scalar_type() == at::kBFloat16 ? GDN_DTYPE_BF16 : GDN_DTYPE_FP16;
 }
 
+constexpr int64_t kMaxToken = 1 << 24;   // token strides of the kernels
+
 // x [B, T, H, P] as the kernels read it in place: a row's heads next to each
 // other, 16-byte aligned rows with strides that are multiples of 8; anything
 // else is copied.
@@ -41,7 +43,7 @@ at::Tensor rows16(const at::Tensor& x) {
     const bool ok = x.stride(3) == 1 && (H <= 1 || x.stride(2) == P) &&
                     (x.size(0) <= 1 || (x.stride(0) % 8 == 0 && x.stride(0) >= 0)) &&
                     (x.size(1) <= 1 || (x.stride(1) % 8 == 0 && x.stride(1) >= 0 &&
-                                        x.stride(1) <= 0x7fffffff)) &&
+                                        x.stride(1) < kMaxToken)) &&
                     reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
     if (ok) return x;
     at::Tensor r = x.contiguous();
@@ -88,7 +90,8 @@ struct Inputs {
                     "head dims are multiples of 16 up to 256 (got ", P, ")");
         TORCH_CHECK(N == 16 || N == 32 || N == 64 || N == 128 || N == 256,
                     "state dims are 16, 32, 64, 128 or 256 (got ", N, ")");
-        TORCH_CHECK(Bn <= 0x7fffffff && T <= 0x40000000 && H <= 0x7fffffff, "too many rows");
+        TORCH_CHECK(Bn <= 0x7fffffff && T <= 0x40000000 && H * P < kMaxToken && G * N < kMaxToken,
+                    "too many rows, or rows of 2^24 elements");
         TORCH_CHECK(dt_min >= 0 && dt_max >= dt_min, "0 <= dt_min <= dt_max");
         if (z_) {
             on_device(*z_, x_, "z");
@@ -100,7 +103,7 @@ struct Inputs {
         c = rows16(c_);
         if (z_) z = rows16(*z_);
         const bool dt_ok = (H <= 1 || dt_.stride(2) == 1) && dt_.stride(0) >= 0 &&
-                           dt_.stride(1) >= 0 && (T <= 1 || dt_.stride(1) <= 0x7fffffff);
+                           dt_.stride(1) >= 0 && (T <= 1 || dt_.stride(1) < kMaxToken);
         dt = dt_ok ? dt_ : dt_.contiguous();
         in.A_log = head_param(A_log_, x_, H, "A_log", A_log);
         in.D = D_ ? head_param(*D_, x_, H, "D", D) : nullptr;
