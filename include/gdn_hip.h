@@ -361,7 +361,8 @@ hipError_t gdn_request_blocks(const int32_t* lengths, const int32_t* slots, int 
 /* gdn_causal_conv1d_fwd that continues from a state and hands one on, for
  * fixed-length or packed sequences.  x, y, w, bias, K, dtypes and silu as
  * there; state0 (or null: zeros) and state are [num_seqs][D][state_len] of
- * io_dtype, oldest token first, state_len in K-1..8, 16-byte aligned; state
+ * io_dtype, oldest token first, state_len in K-1..8; states, w and bias are
+ * 16-byte aligned; state
  * (out) holds the last state_len tokens of state0 followed by the sequence, and
  * must not be state0.  cu_seqlens (B = 1) as in gdn_ssm_scan, or null
  * (num_seqs is B); y rows behind the last sequence are not written.  The sum

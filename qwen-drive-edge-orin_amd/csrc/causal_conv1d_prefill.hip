@@ -7,8 +7,9 @@
 // in front of the activation, as the functions that it stands for do).
 // state[d][p] = r[n - L + p][d], the last L tokens of state0 and sequence.
 //
-// HBM-bound: x once, y once.  A thread owns 8 channels (16 bytes) and a run
-// of kRun consecutive tokens of the row, whose loads are all issued before
+// Bound by HBM (x once, y once) and, next to it, by SiLU's exponential and
+// reciprocal.  A thread owns 8 channels (16 bytes) and a run of kRun consecutive
+// tokens of the row, whose loads are all issued before
 // anything is waited for; neighbouring runs share K - 1 rows (L2).  The
 // sequence of a run's first token comes from a search in cu_seqlens that
 // overlaps those loads (their addresses do not depend on it), and where a
@@ -39,14 +40,39 @@ struct ConvArgs {
     int B, T, D, L, seqs;
     int vecs;        // D / 8
     int runs;        // runs of a batch row
-    int64_t units;   // (B x runs + seqs) x vecs
+    uint32_t units;  // (B x runs + seqs) x vecs
 };
 
 // Work-groups are dealt round-robin to the 8 XCDs: one contiguous range of
 // units per XCD keeps neighbouring runs' shared rows in one L2
-__device__ __forceinline__ int64_t xcd_group(int64_t id, int64_t n) {
-    const int64_t q = n / 8, r = n % 8, xcd = id % 8;
-    return xcd * q + (xcd < r ? xcd : r) + id / 8;
+__device__ __forceinline__ uint32_t xcd_group(uint32_t id, uint32_t n) {
+    const uint32_t q = n / 8, r = n % 8, xcd = id % 8;
+    return xcd * q + min(xcd, r) + id / 8;
+}
+
+// COUNT consecutive parameters (a multiple of 8) at a 16-byte boundary
+template <int WT, int COUNT>
+__device__ __forceinline__ void load_params(const void* p, size_t first, float (&out)[COUNT]) {
+    if constexpr (WT == 2) {
+        const f32x4* v = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + first);
+#pragma unroll
+        for (int i = 0; i < COUNT / 4; ++i) {
+            const f32x4 r = v[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[4 * i + j] = r[j];
+        }
+    } else {
+        const u32x4* v = reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + first);
+#pragma unroll
+        for (int i = 0; i < COUNT / 8; ++i) {
+            const u32x4 r = v[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                out[8 * i + 2 * j] = io_lo<WT>(r[j]);
+                out[8 * i + 2 * j + 1] = io_hi<WT>(r[j]);
+            }
+        }
+    }
 }
 
 __device__ __forceinline__ uint16_t half_of(const u32x4& v, int e) {
@@ -56,11 +82,11 @@ __device__ __forceinline__ uint16_t half_of(const u32x4& v, int e) {
 
 template <int IO, int WT, int K, bool SILU, int kRun>
 __global__ __launch_bounds__(kThreads) void causal_conv1d_prefill_kernel(const ConvArgs a) {
-    const int64_t unit = xcd_group(blockIdx.x, gridDim.x) * kThreads + threadIdx.x;
+    const uint32_t unit = xcd_group(blockIdx.x, gridDim.x) * kThreads + threadIdx.x;
     if (unit >= a.units) return;
-    const int64_t row = unit / a.vecs;
+    const uint32_t row = unit / (uint32_t)a.vecs;
     const int d0 = 8 * (int)(unit - row * a.vecs);
-    const int64_t token_units = (int64_t)a.B * a.runs;
+    const uint32_t token_units = (uint32_t)a.B * a.runs;
 
     if (row >= token_units) {   // the state that sequence s hands on
         const int s = (int)(row - token_units);
@@ -104,8 +130,8 @@ __global__ __launch_bounds__(kThreads) void causal_conv1d_prefill_kernel(const C
         return;
     }
 
-    const int b = (int)(row / a.runs);
-    const int t0 = (int)(row - (int64_t)b * a.runs) * kRun;
+    const int b = (int)(row / (uint32_t)a.runs);
+    const int t0 = (int)(row - (uint32_t)b * a.runs) * kRun;
     const int len = min(kRun, a.T - t0);   // >= 1
     const uint16_t* xb = a.x + b * a.xbs + d0;
     uint16_t* yb = a.y + b * a.ybs + d0;
@@ -117,13 +143,11 @@ __global__ __launch_bounds__(kThreads) void causal_conv1d_prefill_kernel(const C
         const int t = min(max(t0 - (K - 1) + i, 0), t0 + len - 1);
         raw[i] = *reinterpret_cast<const u32x4*>(xb + (size_t)t * a.xts);
     }
-    float wf[8][K], bf[8];
+    float wf[8 * K], bf[8];   // wf[e K + j]
+    load_params<WT>(a.w, (size_t)d0 * K, wf);
+    load_params<WT>(a.bias ? a.bias : a.w, a.bias ? d0 : 0, bf);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-#pragma unroll
-        for (int j = 0; j < K; ++j) wf[e][j] = io_elem<WT>(a.w, (size_t)(d0 + e) * K + j);
-        bf[e] = a.bias ? io_elem<WT>(a.bias, d0 + e) : 0.f;
-    }
+    for (int e = 0; e < 8; ++e) bf[e] = a.bias ? bf[e] : 0.f;
     __builtin_amdgcn_sched_barrier(0);   // every load is issued before the search waits
 
     int s = b, lo = 0, hi = a.T;
@@ -187,12 +211,12 @@ __global__ __launch_bounds__(kThreads) void causal_conv1d_prefill_kernel(const C
                 const int e = 2 * p + q;
                 float acc = bf[e];
 #pragma unroll
-                for (int j = 0; j < K; ++j) acc = fmaf(wf[e][j], win[j][e], acc);
+                for (int j = 0; j < K; ++j) acc = fmaf(wf[e * K + j], win[j][e], acc);
                 v[q] = SILU ? silu_fast(acc) : acc;
             }
             out[p] = io_pack<IO>(v[0], v[1]);
         }
-        *reinterpret_cast<u32x4*>(yb + (size_t)(t0 + i) * a.yts) = out;
+        __builtin_nontemporal_store(out, reinterpret_cast<u32x4*>(yb + (size_t)(t0 + i) * a.yts));
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) {
 #pragma unroll
@@ -204,17 +228,23 @@ __global__ __launch_bounds__(kThreads) void causal_conv1d_prefill_kernel(const C
 template <int IO, int WT, int K, bool SILU, int kRun>
 hipError_t launch_run(ConvArgs& a, hipStream_t stream) {
     a.runs = (a.T + kRun - 1) / kRun;
-    a.units = ((int64_t)a.B * a.runs + a.seqs) * a.vecs;
-    const int64_t groups = (a.units + kThreads - 1) / kThreads;
-    if (groups > 0x7fffffff) return hipErrorInvalidValue;
+    const int64_t units = ((int64_t)a.B * a.runs + a.seqs) * a.vecs;
+    if (units > 0x7fffffff) return hipErrorInvalidValue;
+    a.units = (uint32_t)units;
+    const int64_t groups = (units + kThreads - 1) / kThreads;
     hipLaunchKernelGGL((causal_conv1d_prefill_kernel<IO, WT, K, SILU, kRun>), dim3((unsigned)groups),
                        dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
 
+// Runs of 8 tokens re-read the fewest rows, but leave a short prompt too few
+// waves: below 3 a SIMD, runs of 3 (1141 tokens x 6144 channels: 8.2 us against
+// 9.6; 19,861 packed x 4352: 96.0 against 73.8, which is 4.7 TB/s).
 template <int IO, int WT, int K>
 hipError_t launch(ConvArgs& a, int silu, hipStream_t stream) {
-    return silu ? launch_run<IO, WT, K, true, 8>(a, stream) : launch_run<IO, WT, K, false, 8>(a, stream);
+    const bool wide = (int64_t)a.B * ((a.T + 7) / 8) * a.vecs >= 3 * 1024 * 64;
+    if (silu) return wide ? launch_run<IO, WT, K, true, 8>(a, stream) : launch_run<IO, WT, K, true, 3>(a, stream);
+    return wide ? launch_run<IO, WT, K, false, 8>(a, stream) : launch_run<IO, WT, K, false, 3>(a, stream);
 }
 
 template <int IO, int WT>
@@ -246,7 +276,10 @@ extern "C" hipError_t gdn_causal_conv1d_prefill(const void* x, const void* w, co
     if (!w || !state || state == state0 || (T > 0 && (!x || !y))) return hipErrorInvalidValue;
     if ((x_bstride | x_tstride | y_bstride | y_tstride) % 8 != 0 || x_bstride < 0 ||
         x_tstride < 0 || y_bstride < 0 || y_tstride < 0 ||
-        ((uintptr_t)x | (uintptr_t)y | (uintptr_t)state | (uintptr_t)state0) % 16 != 0)
+        ((uintptr_t)x | (uintptr_t)y | (uintptr_t)state | (uintptr_t)state0 | (uintptr_t)w |
+         (uintptr_t)bias) %
+                16 !=
+            0)
         return hipErrorInvalidValue;
     ConvArgs a{static_cast<const uint16_t*>(x), w, bias, static_cast<const uint16_t*>(state0),
                static_cast<uint16_t*>(y), static_cast<uint16_t*>(state), cu_seqlens, x_bstride,

@@ -60,34 +60,37 @@ __device__ __forceinline__ int group_scan(int v, int top, int* red, int& all) {
     return sat(v, before, top);
 }
 
-// cu[0..N] and start[0..N] by one group
+// cu[0..N] and start[0..N] by one group: a thread adds up `each` consecutive
+// requests, so that the batch takes two scans over the group however long it is
 template <int NT>
 __device__ void form_sums(const int32_t* lens, int N, int total, int block, int* cu, int* start,
                           int* red) {
-    int base = 0, rbase = 0;
-    if (threadIdx.x == 0) cu[0] = start[0] = 0;
-    for (int n0 = 0; n0 < N; n0 += NT) {
-        const int n = n0 + threadIdx.x;
-        const int len = n < N ? min(max(lens[n], 0), total) : 0;
-        int all, rall;
-        const int incl = sat(group_scan<NT>(len, total, red, all), base, total);
-        const int lane_prev = __shfl_up(incl, 1, 64);
-        // the previous request's end: from the neighbouring lane, or its wave's sum
-        int prev = lane_prev;
-        if ((threadIdx.x & 63) == 0) {
-            prev = base;
-            for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) prev = sat(prev, red[w], total);
-        }
-        const int rows = n < N ? rows_of(incl - prev, block) : 0;
-        const int rincl = group_scan<NT>(rows, 0x40000000, red, rall) + rbase;
-        if (n < N) {
-            cu[n + 1] = incl;
-            start[n + 1] = rincl;
-        }
-        base = sat(base, all, total);
-        rbase += rall;
-        __syncthreads();
+    const int each = (N + NT - 1) / NT;
+    const int n0 = min((int)threadIdx.x * each, N), n1 = min(n0 + each, N);
+    auto len = [&](int n) { return min(max(lens[n], 0), total); };
+    int sum = 0, all;
+    for (int n = n0; n < n1; ++n) sum = sat(sum, len(n), total);
+    const int incl = group_scan<NT>(sum, total, red, all);
+    // what lies in front of this thread's requests: its neighbour's sum
+    int before = __shfl_up(incl, 1, 64);
+    if ((threadIdx.x & 63) == 0) {
+        before = 0;
+        for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) before = sat(before, red[w], total);
     }
+    int rows = 0, at = before;
+    for (int n = n0; n < n1; ++n) {
+        const int next = sat(at, len(n), total);
+        rows += rows_of(next - at, block);
+        cu[n + 1] = at = next;
+    }
+    int row = group_scan<NT>(rows, 0x40000000, red, all) - rows;
+    at = before;
+    for (int n = n0; n < n1; ++n) {
+        const int next = sat(at, len(n), total);
+        start[n + 1] = row += rows_of(next - at, block);
+        at = next;
+    }
+    if (threadIdx.x == 0) cu[0] = start[0] = 0;
     __syncthreads();
 }
 

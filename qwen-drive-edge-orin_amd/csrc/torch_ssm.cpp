@@ -33,6 +33,12 @@ int io_dtype(const at::Tensor& x) {
     return x.scalar_type() == at::kBFloat16 ? GDN_DTYPE_BF16 : GDN_DTYPE_FP16;
 }
 
+// x without gaps at a 16-byte boundary, itself where it lies so
+at::Tensor aligned16(const at::Tensor& x) {
+    at::Tensor r = x.contiguous();
+    return reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0 ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+
 constexpr int64_t kMaxToken = 1 << 24;   // token strides of the kernels
 
 // x [B, T, H, P] as the kernels read it in place: a row's heads next to each
@@ -45,9 +51,7 @@ at::Tensor rows16(const at::Tensor& x) {
                     (x.size(1) <= 1 || (x.stride(1) % 8 == 0 && x.stride(1) >= 0 &&
                                         x.stride(1) < kMaxToken)) &&
                     reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
-    if (ok) return x;
-    at::Tensor r = x.contiguous();
-    return reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0 ? r : r.clone(at::MemoryFormat::Contiguous);
+    return ok ? x : aligned16(x);
 }
 
 // fp32 [H] parameters
@@ -278,9 +282,7 @@ std::vector<at::Tensor> causal_conv1d_prefill(const at::Tensor& x, const at::Ten
                     "state0 must be [N, D, L] in the dtype of x");
         TORCH_CHECK(state_len == 0 || state_len == state0->size(2), "state0 must have state_len columns");
         state_len = state0->size(2);
-        s0c = state0->contiguous();
-        if (reinterpret_cast<uintptr_t>(s0c.data_ptr()) % 16 != 0)
-            s0c = s0c.clone(at::MemoryFormat::Contiguous);
+        s0c = aligned16(*state0);
     }
     if (state_len == 0) state_len = K;
     TORCH_CHECK(state_len >= K - 1 && state_len <= 8, "state_len must be K - 1 .. 8");
@@ -289,9 +291,9 @@ std::vector<at::Tensor> causal_conv1d_prefill(const at::Tensor& x, const at::Ten
                         (T <= 1 || (xt.stride(1) % 8 == 0 && xt.stride(1) >= 0)) &&
                         reinterpret_cast<uintptr_t>(xt.data_ptr()) % 16 == 0;
     if (!direct) xt = xt.contiguous();
-    auto wc = weight.contiguous();
+    auto wc = aligned16(weight);
     at::Tensor bc;
-    if (bias) bc = bias->contiguous();
+    if (bias) bc = aligned16(*bias);
     auto yt = at::empty({B, T, D}, x.options());
     auto state = at::empty({seqs, D, state_len}, x.options());
     check_hip(gdn_causal_conv1d_prefill(
@@ -362,8 +364,7 @@ at::Tensor as_rows(const at::Tensor& x, int64_t C, int64_t& stride) {
         want = x.stride(d) * x.size(d);
     }
     if (!ok) {
-        r = x.contiguous();
-        if (reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 != 0) r = r.clone(at::MemoryFormat::Contiguous);
+        r = aligned16(x);
         step = C;
     }
     stride = step < 0 ? C : step;
@@ -390,8 +391,7 @@ at::Tensor gated_groupnorm(const at::Tensor& x, const at::Tensor& z, const at::T
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     int64_t xs = C, zs = C;
     auto xr = as_rows(x, C, xs), zr = as_rows(z, C, zs);
-    auto wc = weight.contiguous();
-    if (reinterpret_cast<uintptr_t>(wc.data_ptr()) % 16 != 0) wc = wc.clone(at::MemoryFormat::Contiguous);
+    auto wc = aligned16(weight);
     auto y = at::empty(x.sizes(), x.options());
     check_hip(gdn_gated_groupnorm_forward(
                   xr.data_ptr(), xs, zr.data_ptr(), zs, wc.data_ptr(), y.data_ptr(), x.numel() / C,
