@@ -39,6 +39,11 @@ namespace gdn {
 namespace {
 
 constexpr int kMaxBlock = 1 << 20;
+// Segments of a fixed-length sequence that the main pass joins by itself: each
+// group reads the records in front of its own, which is less than a launch of
+// the join up to here (1141 tokens x 64 heads in 6
+// segments: 38 us against 41; 4 x 2048 tokens x 32 in 8: 95 against 82)
+constexpr int kMaxFold = 6;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kTiles = 2;          // 16-column tiles of a wave
@@ -60,6 +65,7 @@ struct ScanArgs {
     int segs, seqs, block;
     int slices;          // column slices of a head: ceil(P / PW)
     int tasks;           // slices of a group: heads / groups x slices
+    bool fold;           // the main pass joins the segments' states itself
     int quads;           // work-groups per group and segment: ceil(tasks / waves)
     f32x4* states;       // [row][group][task] fragments of a slice's state
     float* decays;       // [row][group][task]
@@ -333,7 +339,7 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
 #pragma unroll
         for (int pt = 0; pt < PT; ++pt) S[nt][pt] = zero4();
     const size_t hs = ((size_t)s.seq * H + h) * N * P;
-    const size_t rec = ((size_t)row * in.groups + grp) * a.tasks + tk;   // state record
+    const int64_t rec = ((int64_t)row * in.groups + grp) * a.tasks + tk;   // state record
     // element (nt, pt, i) of a lane in a state [N][P]: so + n_off(nt, i) P + p_off(pt)
     const size_t so = hs + (size_t)(8 * g) * P + p0 + 8 * (m >> 2) + (m & 3);
     auto n_off = [](int nt, int i) { return 32 * (nt >> 1) + 4 * (nt & 1) + i; };
@@ -352,11 +358,21 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
                 }
         }
     } else if (!kLocal) {
-        const f32x4* from = a.states + (rec - (size_t)in.groups * a.tasks) * (NT * PT * 64) + lane;
+        // the record of the segment in front, joined already, or (few segments)
+        // the segments' own, joined here
+        const int64_t all = (int64_t)in.groups * a.tasks;
+        const int count = a.fold ? min(s.idx, kMaxFold - 1) : 1;
+        for (int k = count; k > 0; --k) {
+            const f32x4* from = a.states + (rec - k * all) * (NT * PT * 64) + lane;
+            const float decay = k < count ? a.decays[rec - k * all] : 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int pt = 0; pt < PT; ++pt) S[nt][pt] = from[(nt * PT + pt) * 64];
+                for (int pt = 0; pt < PT; ++pt) {
+                    const f32x4 L = from[(nt * PT + pt) * 64];
+                    S[nt][pt] = k < count ? S[nt][pt] * decay + L : L;
+                }
+        }
     }
 
     const float A2 = -expf(in.A_log[h]) * kLog2e;
@@ -869,7 +885,7 @@ hipError_t launch_scan(const ScanArgs& a, hipStream_t stream) {
         hipLaunchKernelGGL((ssm_scan_kernel<IO, N, PT, WAVES, true>), dim3((unsigned)groups),
                            dim3(64 * WAVES), 0, stream, a);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-        if (a.table || a.segs > 2) {
+        if (a.table || a.segs > kMaxFold) {
             // 16 bytes a thread from 2^17 such threads on (8 sequences of 2..7
             // segments x 128 records: 13 us against 35 with 4 bytes; one of 64
             // segments x 32 records: 30 us against 15)
@@ -956,11 +972,15 @@ extern "C" int gdn_ssm_scan_block(const gdn_ssm_inputs* in, int num_seqs) {
     double least = 0;
     for (int c = 1; c <= kMaxBlock / kChunk; c += c < 16 ? 1 : c / 8) {
         const double segs = packed ? std::max(1.0, per_seq / c + 0.5) : std::ceil(per_seq / c);
-        double us = passes_us(num_seqs * segs * units, std::min<double>(c, longest), deep, main_t, 5) * scale;
+        double us = passes_us(num_seqs * segs * units, std::min<double>(c, longest), deep, main_t, 4) * scale;
         if (segs > 1)
             us += 3 + passes_us(num_seqs * (segs - 1) * units, std::min<double>(c, longest), local_deep, local_t,
                                 4) * scale;
-        if (segs > 2) us += 4 + 2 * num_seqs * (segs - 2) * record_us;
+        // records: written by the first pass, and read by the main pass (all
+        // in front of a segment, where it joins them) or the join
+        const bool fold = !packed && segs <= kMaxFold;
+        us += num_seqs * (segs - 1) * record_us * (fold ? 1 + segs / 2 : 2);
+        if (segs > 2 && !fold) us += 4 + 2 * num_seqs * (segs - 2) * record_us;
         if (c == 1 || us < least) {
             least = us;
             best = c;
@@ -1004,6 +1024,7 @@ extern "C" hipError_t gdn_ssm_scan(const gdn_ssm_inputs* in, void* y, const floa
     a.slices = l.slices;
     a.tasks = l.tasks;
     a.quads = l.quads;
+    a.fold = !packed && l.segs <= kMaxFold;
     a.states = reinterpret_cast<f32x4*>(ws + l.states);
     a.decays = reinterpret_cast<float*>(ws + l.decays);
     if (packed) {
