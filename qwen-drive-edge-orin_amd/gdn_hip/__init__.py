@@ -117,6 +117,8 @@ def causal_conv1d_fwd(x, weight, bias=None, silu=False):
 
 
 def causal_conv1d_update(x, conv_state, weight, bias=None, silu=False, *, slots=None):
+    if slots is None:
+        return load().causal_conv1d_update(x, conv_state, weight, bias, silu)
     return load().causal_conv1d_update(x, conv_state, weight, bias, silu, slots=slots)
 
 

@@ -12,9 +12,12 @@ x is ``[B, D, T]`` (the update also takes ``[B, D]``), weight ``[D, K]`` or
 with L in K-1..8 (updated in place).  x must be bf16 or fp16 and weight/bias
 of x's dtype or fp32.  Outputs match the torch fallbacks' dtype steps: the
 convolution in the weight dtype with an fp32 sum, SiLU in fp32, rounded to
-x's dtype.  Features the kernels do not implement (``seq_idx``, initial or
-final states of the prefill form, ``cache_seqlens``, ``conv_state_indices``,
-activations other than SiLU) raise; there is no silent fallback.
+x's dtype.  With initial states or asked for final ones, ``causal_conv1d_fn``
+runs the form that carries them (one rounding, at the end; states ``[B, D,
+K - 1]``), and ``conv_state_indices`` ``[B]`` makes conv_state a pool (an index
+outside it is a row without a request: zeros, no state changes).  Features the
+kernels do not implement (``seq_idx``, ``cache_seqlens``, activations other
+than SiLU) raise; there is no silent fallback.
 """
 from __future__ import annotations
 
@@ -55,23 +58,34 @@ def _on_device(**tensors):
 def causal_conv1d_fn(x, weight, bias=None, seq_idx=None, initial_states=None,
                      return_final_states=False, final_states_out=None, activation=None):
     """Causal depthwise conv1d over x [B, D, T]; returns [B, D, T] in x's
-    dtype (a transposed view of a contiguous [B, T, D] buffer)."""
-    if seq_idx is not None or initial_states is not None or return_final_states or \
-            final_states_out is not None:
-        raise NotImplementedError("seq_idx / initial_states / final states are not supported")
+    dtype (a transposed view of a contiguous [B, T, D] buffer), and with
+    return_final_states the pair of it and the last K - 1 tokens [B, D, K - 1]
+    (in final_states_out where that is given)."""
+    if seq_idx is not None:
+        raise NotImplementedError("seq_idx is not supported")
     silu = _silu(activation)
-    _on_device(x=x, weight=weight, bias=bias)
+    _on_device(x=x, weight=weight, bias=bias, initial_states=initial_states,
+               final_states_out=final_states_out)
     if x.dim() != 3:
         raise ValueError("x must be [B, D, T]")
-    return gdn_hip.causal_conv1d_fwd(x, _weight(weight), bias, silu)
+    weight = _weight(weight)
+    if initial_states is None and not return_final_states:
+        return gdn_hip.causal_conv1d_fwd(x, weight, bias, silu)
+    y, final = gdn_hip.causal_conv1d_prefill(x, weight, bias, initial_states, silu=silu,
+                                             state_len=weight.shape[1] - 1)
+    if not return_final_states:
+        return y
+    if final_states_out is not None:
+        final = final_states_out.copy_(final)
+    return y, final
 
 
 def causal_conv1d_update(x, conv_state, weight, bias=None, activation=None, cache_seqlens=None,
                          conv_state_indices=None):
     """Decode step: x [B, D, T] or [B, D] is appended to conv_state (updated
     in place); returns the outputs for x's tokens in x's shape and dtype."""
-    if cache_seqlens is not None or conv_state_indices is not None:
-        raise NotImplementedError("cache_seqlens / conv_state_indices are not supported")
+    if cache_seqlens is not None:
+        raise NotImplementedError("cache_seqlens is not supported")
     silu = _silu(activation)
     _on_device(x=x, conv_state=conv_state, weight=weight, bias=bias)
     squeeze = x.dim() == 2
@@ -79,5 +93,9 @@ def causal_conv1d_update(x, conv_state, weight, bias=None, activation=None, cach
         x = x.unsqueeze(-1)
     if x.dim() != 3:
         raise ValueError("x must be [B, D, T] or [B, D]")
-    y = gdn_hip.causal_conv1d_update(x, conv_state, _weight(weight), bias, silu)
+    if conv_state_indices is None:
+        y = gdn_hip.causal_conv1d_update(x, conv_state, _weight(weight), bias, silu)
+    else:
+        y = gdn_hip.causal_conv1d_update(x, conv_state, _weight(weight), bias, silu,
+                                         slots=conv_state_indices)
     return y.squeeze(-1) if squeeze else y
