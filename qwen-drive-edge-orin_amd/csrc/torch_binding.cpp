@@ -538,20 +538,18 @@ at::Tensor causal_conv1d_fwd(const at::Tensor& x, const at::Tensor& weight,
 }
 
 // x: [B, D, T] (any strides), conv_state: [B, D, L] with unit token stride,
-// updated in place; weight [D, K]; bias [D] or None; slots [B] or None: the
-// states are a pool and row b uses slots[b].  Returns y [B, D, T]
+// updated in place; weight [D, K]; bias [D] or None.  Returns y [B, D, T]
 // laid out like causal_conv1d_fwd's.
 at::Tensor causal_conv1d_update(const at::Tensor& x, at::Tensor conv_state,
                                 const at::Tensor& weight, const std::optional<at::Tensor>& bias,
-                                bool silu, const std::optional<at::Tensor>& slots) {
+                                bool silu) {
     TORCH_CHECK(x.is_cuda() && conv_state.is_cuda() && weight.is_cuda() &&
                     (!bias || bias->is_cuda()),
                 "all inputs must be CUDA tensors");
     TORCH_CHECK(x.dim() == 3, "x must be [B, D, T]");
     const int64_t B = x.size(0), D = x.size(1), T = x.size(2);
-    TORCH_CHECK(conv_state.dim() == 3 && (slots || conv_state.size(0) == B) &&
-                    conv_state.size(1) == D,
-                "conv_state must be [B (or slots), D, L]");
+    TORCH_CHECK(conv_state.dim() == 3 && conv_state.size(0) == B && conv_state.size(1) == D,
+                "conv_state must be [B, D, L]");
     TORCH_CHECK(conv_state.scalar_type() == x.scalar_type(), "conv_state must have the dtype of x");
     TORCH_CHECK(conv_state.stride(2) == 1 || conv_state.size(2) == 1,
                 "conv_state must have unit stride along its last dimension");
@@ -563,23 +561,6 @@ at::Tensor causal_conv1d_update(const at::Tensor& x, at::Tensor conv_state,
     std::optional<at::Tensor> bc;
     if (bias) bc = bias->contiguous();
     auto y = at::empty({B, T, D}, x.options()).transpose(1, 2);
-    if (slots) {
-        TORCH_CHECK(slots->is_cuda() && slots->device() == x.device() && slots->dim() == 1 &&
-                        slots->size(0) == B &&
-                        (slots->scalar_type() == at::kInt || slots->scalar_type() == at::kLong),
-                    "slots must be int32 or int64 [B] on x's device");
-        TORCH_CHECK(conv_state.size(0) >= 1 && conv_state.size(0) <= 0x7fffffff, "bad pool size");
-        auto sl = slots->to(at::kInt).contiguous();
-        check_hip(gdn_causal_conv1d_update_slots(
-                      x.data_ptr(), conv_state.data_ptr(), wc.data_ptr(),
-                      bc ? bc->data_ptr() : nullptr, y.data_ptr(), sl.data_ptr<int32_t>(),
-                      (int)conv_state.size(0), (int)B, (int)T, (int)D, (int)wc.size(1),
-                      (int)conv_state.size(2), x.stride(0), x.stride(2), x.stride(1),
-                      conv_state.stride(0), conv_state.stride(1), y.stride(0), y.stride(2),
-                      y.stride(1), io, wd, silu ? 1 : 0, current_stream()),
-                  "gdn_causal_conv1d_update_slots");
-        return y;
-    }
     check_hip(gdn_causal_conv1d_update(x.data_ptr(), conv_state.data_ptr(), wc.data_ptr(),
                                        bc ? bc->data_ptr() : nullptr, y.data_ptr(), (int)B, (int)T,
                                        (int)D, (int)wc.size(1), (int)conv_state.size(2),
@@ -587,6 +568,45 @@ at::Tensor causal_conv1d_update(const at::Tensor& x, at::Tensor conv_state,
                                        conv_state.stride(1), y.stride(0), y.stride(2), y.stride(1),
                                        io, wd, silu ? 1 : 0, current_stream()),
               "gdn_causal_conv1d_update");
+    return y;
+}
+
+// The same on a pool of states: conv_state [slots, D, L], row b uses slots[b].
+at::Tensor causal_conv1d_update_slots(const at::Tensor& x, at::Tensor conv_state,
+                                      const at::Tensor& weight,
+                                      const std::optional<at::Tensor>& bias, bool silu,
+                                      const at::Tensor& slots) {
+    TORCH_CHECK(x.is_cuda() && conv_state.is_cuda() && weight.is_cuda() &&
+                    (!bias || bias->is_cuda()),
+                "all inputs must be CUDA tensors");
+    TORCH_CHECK(x.dim() == 3, "x must be [B, D, T]");
+    const int64_t B = x.size(0), D = x.size(1), T = x.size(2);
+    TORCH_CHECK(conv_state.dim() == 3 && conv_state.size(1) == D && conv_state.size(0) >= 1 &&
+                    conv_state.size(0) <= 0x7fffffff,
+                "conv_state must be [slots, D, L]");
+    TORCH_CHECK(conv_state.scalar_type() == x.scalar_type(), "conv_state must have the dtype of x");
+    TORCH_CHECK(conv_state.stride(2) == 1 || conv_state.size(2) == 1,
+                "conv_state must have unit stride along its last dimension");
+    TORCH_CHECK(weight.dim() == 2 && weight.size(0) == D, "weight must be [D, K]");
+    TORCH_CHECK(!bias || (bias->dim() == 1 && bias->size(0) == D), "bias must be [D]");
+    TORCH_CHECK(slots.is_cuda() && slots.device() == x.device() && slots.dim() == 1 &&
+                    slots.size(0) == B &&
+                    (slots.scalar_type() == at::kInt || slots.scalar_type() == at::kLong),
+                "slots must be int32 or int64 [B] on x's device");
+    const int io = conv_io_dtype(x), wd = conv_w_dtype(x, weight, bias);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    auto wc = weight.contiguous();
+    std::optional<at::Tensor> bc;
+    if (bias) bc = bias->contiguous();
+    auto sl = slots.to(at::kInt).contiguous();
+    auto y = at::empty({B, T, D}, x.options()).transpose(1, 2);
+    check_hip(gdn_causal_conv1d_update_slots(
+                  x.data_ptr(), conv_state.data_ptr(), wc.data_ptr(), bc ? bc->data_ptr() : nullptr,
+                  y.data_ptr(), sl.data_ptr<int32_t>(), (int)conv_state.size(0), (int)B, (int)T,
+                  (int)D, (int)wc.size(1), (int)conv_state.size(2), x.stride(0), x.stride(2),
+                  x.stride(1), conv_state.stride(0), conv_state.stride(1), y.stride(0), y.stride(2),
+                  y.stride(1), io, wd, silu ? 1 : 0, current_stream()),
+              "gdn_causal_conv1d_update_slots");
     return y;
 }
 
@@ -635,6 +655,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "x"_a, "weight"_a, "bias"_a = std::nullopt, "silu"_a = false);
     m.def("causal_conv1d_update", &causal_conv1d_update,
           "decode-time causal conv1d; conv_state [B, D, L] updated in place; returns y", "x"_a,
-          "conv_state"_a, "weight"_a, "bias"_a = std::nullopt, "silu"_a = false,
-          pybind11::kw_only(), "slots"_a = std::nullopt);
+          "conv_state"_a, "weight"_a, "bias"_a = std::nullopt, "silu"_a = false);
+    m.def("causal_conv1d_update_slots", &causal_conv1d_update_slots,
+          "causal_conv1d_update on a pool of states [slots, D, L]: row b uses slots[b], a slot "
+          "outside the pool is a row without a request (zeros)",
+          "x"_a, "conv_state"_a, "weight"_a, "bias"_a, "silu"_a, "slots"_a);
 }

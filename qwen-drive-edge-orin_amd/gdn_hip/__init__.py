@@ -119,7 +119,7 @@ def causal_conv1d_fwd(x, weight, bias=None, silu=False):
 def causal_conv1d_update(x, conv_state, weight, bias=None, silu=False, *, slots=None):
     if slots is None:
         return load().causal_conv1d_update(x, conv_state, weight, bias, silu)
-    return load().causal_conv1d_update(x, conv_state, weight, bias, silu, slots=slots)
+    return load().causal_conv1d_update_slots(x, conv_state, weight, bias, silu, slots)
 
 
 def ssm_scan(x, dt, A_log, B, C, D=None, z=None, dt_bias=None, s0=None, *, cu_seqlens=None,
