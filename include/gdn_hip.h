@@ -324,8 +324,9 @@ hipError_t gdn_ssm_step(const gdn_ssm_inputs* in, void* y, float* state, const i
  * batch).  cu_seqlens int32 [num_seqs + 1]: batch is 1 and the row holds
  * packed sequences (clamped as in deltanet_chunk_prefill_varlen; y rows behind
  * the last sequence are not written).  s0 (or null: zeros) and sf are fp32
- * [num_seqs][heads][state_dim][head_dim]; sf may be s0.  A sequence without
- * tokens hands its state on.  blocks (or null): gdn_request_blocks' table for
+ * [num_seqs][heads][state_dim][head_dim], which must not overlap (a segment may
+ * still read s0 when another one's end is written).  A sequence without tokens
+ * hands its state on.  blocks (or null): gdn_request_blocks' table for
  * the same cu_seqlens and this `block`; without it a packed call forms the
  * table itself in the workspace.  `block` is the run of tokens that is worked
  * on at a time, a multiple of 64, normally gdn_ssm_scan_block's; results for

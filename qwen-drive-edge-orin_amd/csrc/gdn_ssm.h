@@ -14,10 +14,12 @@ namespace gdn {
 // fp32 ulps for any size of e^x: e^x from the base-2 exponential of x log2(e)
 // in two parts, log1p(e) = log(u) e / (u - 1) with u = fl(1 + e), in which the
 // rounding of u cancels (Goldberg, "What every computer scientist should know
-// about floating-point arithmetic", theorem 4).  Above 20, log1p(e^x) is x.
+// about floating-point arithmetic", theorem 4).  Above 20, log1p(e^x) is x;
+// below -104, -infinity among it, e^x is 0 in fp32.  NaN stays NaN (the
+// comparisons are written so that it does).
 __device__ __forceinline__ float ssm_delta(float raw, float bias, float lo, float hi) {
     const float x = raw + bias;
-    const float y = fminf(x, 20.f);
+    const float y = x > 20.f ? 20.f : x < -104.f ? -104.f : x;
     constexpr float kL = 1.44269502f, kLlo = 1.92596303e-08f;   // log2(e) and what it rounds off
     const float t = y * kL, r = fmaf(y, kLlo, fmaf(y, kL, -t));
     const float e0 = __builtin_amdgcn_exp2f(t);
@@ -25,7 +27,7 @@ __device__ __forceinline__ float ssm_delta(float raw, float bias, float lo, floa
     const float u = 1.f + e, v = u - 1.f;
     const float q = __builtin_amdgcn_logf(u) * 0.693147182f * (e / v);
     const float d = x > 20.f ? x : v == 0.f ? e : q;
-    return fminf(fmaxf(d, lo), hi);
+    return d < lo ? lo : d > hi ? hi : d;
 }
 
 inline bool ssm_aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }

@@ -390,7 +390,7 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
     // start and from its end
     auto token_vectors = [&](float raw, int n) {
         const float d = lane < n ? ssm_delta(raw, bias, in.dt_min, in.dt_max) : 0.f;
-        const float l2 = fmaxf(A2 * d, -150.f);
+        const float l2 = lane < n ? fmaxf(A2 * d, -150.f) : 0.f;
         const float c2 = lane_prefix(l2);
         // lane i of the reversed order is token 63 - i
         const float back = lane_prefix(__shfl(l2, 63 - lane, 64));
@@ -636,8 +636,8 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
             const uint16_t xm = top[0] > top[1] ? top[0] : top[1];
             const float wx_max = wave_max(fabsf((float)__builtin_bit_cast(_Float16, xm))) * w_max;
             const int next_kappa = fit_fp16(fmaxf(dec * s_max * pow2(-kappa), wx_max));
-            // (their difference may pass 2^127 where the state is 0 or decays to nothing)
-            dec = dec * s_max == 0.f ? 0.f : dec * pow2(min(next_kappa - kappa, 127));
+            // (a state that is 0 takes any scale, one 2^126 below w x is nothing)
+            dec = dec * s_max == 0.f ? 0.f : dec * pow2(min(max(next_kappa - kappa, -126), 127));
             kappa = next_kappa;
             w_scale = pow2(kappa);
         }
@@ -843,10 +843,9 @@ bool scan_sizes_ok(const gdn_ssm_inputs* in, int seqs, int block, bool packed) {
            (packed ? in->batch == 1 : seqs == in->batch);
 }
 
-// Whether the chunked scan has an instance; the rest takes the recurrence
-bool chunked(const gdn_ssm_inputs* in) {
-    return in->state_dim >= 64;
-}
+// Whether the chunked scan has an instance (an MFMA sums over 32 state rows);
+// a state of 16 rows takes the recurrence
+bool chunked(const gdn_ssm_inputs* in) { return in->state_dim >= 32; }
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
@@ -907,6 +906,7 @@ hipError_t launch_scan(const ScanArgs& a, hipStream_t stream) {
 template <int IO>
 hipError_t launch_any(const ScanArgs& a, hipStream_t stream) {
     switch (a.in.state_dim) {
+        case 32: return launch_scan<IO, 32, kTiles, kWaves>(a, stream);
         case 64: return launch_scan<IO, 64, kTiles, kWaves>(a, stream);
         case 128: return launch_scan<IO, 128, kTiles, kWaves>(a, stream);
         default: return launch_scan<IO, 256, kTiles, kWaves>(a, stream);
@@ -1004,7 +1004,7 @@ extern "C" hipError_t gdn_ssm_scan(const gdn_ssm_inputs* in, void* y, const floa
     const bool packed = cu_seqlens != nullptr;
     if (!ssm_inputs_ok(in) || !scan_sizes_ok(in, num_seqs, block, packed) || (blocks && !packed))
         return hipErrorInvalidValue;
-    if (!sf || !ssm_aligned(sf, 4) || !ssm_aligned(s0, 4) || (in->tokens > 0 && !y) ||
+    if (!sf || sf == s0 || !ssm_aligned(sf, 4) || !ssm_aligned(s0, 4) || (in->tokens > 0 && !y) ||
         !ssm_aligned(y, 16) || !ssm_aligned(workspace, 256) || !ssm_aligned(blocks, 16))
         return hipErrorInvalidValue;
     const size_t need = gdn_ssm_scan_workspace_size(in, num_seqs, block, packed);

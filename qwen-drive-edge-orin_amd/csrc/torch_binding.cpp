@@ -598,7 +598,9 @@ at::Tensor causal_conv1d_update_slots(const at::Tensor& x, at::Tensor conv_state
     auto wc = weight.contiguous();
     std::optional<at::Tensor> bc;
     if (bias) bc = bias->contiguous();
-    auto sl = slots.to(at::kInt).contiguous();
+    // (what passes 32 bits stays outside any pool)
+    auto sl = slots.scalar_type() == at::kLong ? slots.clamp(-1, 0x7fffffff).to(at::kInt)
+                                               : slots.contiguous();
     auto y = at::empty({B, T, D}, x.options()).transpose(1, 2);
     check_hip(gdn_causal_conv1d_update_slots(
                   x.data_ptr(), conv_state.data_ptr(), wc.data_ptr(), bc ? bc->data_ptr() : nullptr,

@@ -8,6 +8,7 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <limits>
 #include <optional>
 #include <vector>
 
@@ -151,6 +152,16 @@ at::Tensor cu_int32(const at::Tensor& cu, const at::Tensor& x) {
     return cu.to(at::kInt).contiguous();
 }
 
+// slots int32 or int64 [n] as int32; what passes 32 bits stays outside any pool
+at::Tensor slots_int32(const at::Tensor& slots, const at::Tensor& x, int64_t n) {
+    on_device(slots, x, "slots");
+    TORCH_CHECK((slots.scalar_type() == at::kInt || slots.scalar_type() == at::kLong) &&
+                    slots.dim() == 1 && slots.size(0) == n,
+                "slots must be int32 or int64, one per row");
+    return slots.scalar_type() == at::kLong ? slots.clamp(-1, 0x7fffffff).to(at::kInt)
+                                            : slots.contiguous();
+}
+
 // [y, final_state]
 std::vector<at::Tensor> ssm_scan(const at::Tensor& x, const at::Tensor& dt, const at::Tensor& A_log,
                                  const at::Tensor& b, const at::Tensor& c, const OptTensor& D,
@@ -202,6 +213,8 @@ std::vector<at::Tensor> ssm_scan(const at::Tensor& x, const at::Tensor& dt, cons
 // The block that ssm_scan works on for these sizes (host arithmetic)
 int64_t ssm_scan_block(int64_t tokens, int64_t batch, int64_t heads, int64_t head_dim,
                        int64_t groups, int64_t state_dim, int64_t num_seqs) {
+    for (int64_t v : {batch, heads, head_dim, groups, state_dim, num_seqs})
+        TORCH_CHECK(v >= 1 && v <= 0x40000000, "unsupported scan configuration");
     gdn_ssm_inputs in{};
     in.batch = (int)batch;
     in.heads = (int)heads;
@@ -231,12 +244,8 @@ at::Tensor ssm_step(const at::Tensor& x, const at::Tensor& dt, const at::Tensor&
                 "state must be [B (or slots), H, state, head]");
     at::Tensor sl;
     if (slots) {
-        on_device(*slots, x, "slots");
-        TORCH_CHECK((slots->scalar_type() == at::kInt || slots->scalar_type() == at::kLong) &&
-                        slots->dim() == 1 && slots->size(0) == a.in.batch,
-                    "slots must be int32 or int64 [B]");
         TORCH_CHECK(state.size(0) >= 1 && state.size(0) <= 0x7fffffff, "bad pool size");
-        sl = slots->to(at::kInt).contiguous();
+        sl = slots_int32(*slots, x, a.in.batch);
     }
     auto y = at::empty({a.in.batch, a.in.tokens, a.in.heads, a.in.head_dim}, a.x.options());
     check_hip(gdn_ssm_step(&a.in, y.data_ptr(), state.data_ptr<float>(),
@@ -324,13 +333,7 @@ std::vector<at::Tensor> request_blocks(const at::Tensor& lengths, int64_t total_
     at::Tensor len = lengths.scalar_type() == at::kLong ? lengths.clamp(0, total_tokens).to(at::kInt)
                                                         : lengths.contiguous();
     at::Tensor sl;
-    if (slots) {
-        on_device(*slots, lengths, "slots");
-        TORCH_CHECK((slots->scalar_type() == at::kInt || slots->scalar_type() == at::kLong) &&
-                        slots->dim() == 1 && slots->numel() == N,
-                    "slots must be int32 or int64 [N]");
-        sl = slots->to(at::kInt).contiguous();
-    }
+    if (slots) sl = slots_int32(*slots, lengths, N);
     const auto opt = lengths.options().dtype(at::kInt);
     const int64_t rows = gdn_request_block_rows((int)total_tokens, (int)N, (int)block);
     auto sums = at::empty({2, N + 1}, opt);

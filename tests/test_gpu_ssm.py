@@ -115,6 +115,89 @@ def test_scan_packed_with_a_table(dev):
     assert torch.equal(y0, y1) and torch.equal(s0, s1)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("T,H,N", [(1250, 2, 64), (1250, 1, 256)])
+def test_scan_many_segments(dev, T, H, N, dtype):
+    """More segments than the main pass joins by itself."""
+    assert gdn_hip.ssm_scan_block(T, 1, H, 64, 1, N, 1) * 6 < T
+    d = sc.inputs(T, 1, T, H, 64, 1, N, dtype)
+    d["dt_bias"] = d["dt_bias"] - 3
+    _check_scan(dev, d, _s0(T, 1, H, N, 64), dtype, f"scan T={T} N={N} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_scan_many_segments_packed(dev, dtype):
+    """Sequences of up to 9 segments in a table of 64-token blocks, enough
+    records that the join takes 16 bytes a thread."""
+    lengths = [520, 0, 410, 64, 65, 129]
+    T, n = sum(lengths), len(lengths)
+    d = sc.inputs(T, 1, T, 16, 64, 2, 128, dtype)
+    d["dt_bias"] = d["dt_bias"] - 3
+    s0 = _s0(n, n, 16, 128, 64)
+    y, S, ya, Sa = orc.ssm_packed(lengths, **{k: d[k] for k in ("x", "dt", "A_log", "B", "C", "D", "z", "dt_bias")}, s0=s0)
+    g = sc.to(d, dev)
+    cu, table, _, _ = gdn_hip.request_blocks(torch.tensor(lengths, device=dev), T)
+    print(f"packed segments {dtype}", flush=True)
+    oy, oS = gdn_hip.ssm_scan(g["x"], g["dt"], g["A_log"], g["B"], g["C"], g["D"], g["z"],
+                              g["dt_bias"], s0.to(dev), cu_seqlens=cu, blocks=table, block=64)
+    torch.cuda.synchronize()
+    by, bS = sc.bounds(d, max(lengths), y, ya, Sa, dtype)
+    sc.close(oy, y, by, "packed segments y")
+    sc.close(oS, S, bS, "packed segments state")
+
+
+def test_scan_more_sequences_than_one_group_sums(dev):
+    """Past 4096 sequences the table takes two launches."""
+    lengths = [1 + (i % 3) for i in range(4100)]
+    T = sum(lengths)
+    d = sc.to(sc.inputs(3, 1, T, 1, 16, 1, 64, z=False), dev)
+    args = [d[k] for k in ("x", "dt", "A_log", "B", "C", "D", "z", "dt_bias")]
+    y, s = gdn_hip.ssm_scan(*args, cu_seqlens=_cu(lengths, dev))
+    torch.cuda.synchronize()
+    # sequences of one length as a batch
+    cuts = torch.tensor([0] + lengths).cumsum(0)
+    for n in (1, 2, 3):
+        ids = [i for i, m in enumerate(lengths) if m == n]
+        rows = torch.stack([torch.arange(int(cuts[i]), int(cuts[i]) + n) for i in ids]).to(dev)
+        part = [a[0][rows] if a is not None and a.dim() > 1 else a for a in args]
+        yb, sb = gdn_hip.ssm_scan(*part)
+        torch.cuda.synchronize()
+        assert torch.equal(y[0][rows], yb) and torch.equal(s[ids], sb)
+
+
+def test_infinite_and_nan_steps(dev):
+    """dt of -infinity or the type's lowest value is a step of 0 (the token
+    changes nothing); NaN shows in the outputs from its token on."""
+    for dtype in (BF, HF):
+        d = sc.inputs(21, 1, 70, 2, 64, 1, 64, dtype)
+        d["dt"] = d["dt"].clone()
+        d["dt"][:, 20] = -float("inf")
+        d["dt"][:, 40] = torch.finfo(dtype).min
+        _check_scan(dev, d, _s0(2, 1, 2, 64, 64), dtype, f"masked steps {dtype}")
+        g = sc.to(d, dev)
+        st, fin = _s0(2, 1, 2, 64, 64).to(dev), None
+        args = [g[k][:, 20:21] for k in ("x", "dt")] + [g["A_log"]] + [g[k][:, 20:21] for k in ("B", "C")]
+        before = st.clone()
+        gdn_hip.ssm_step(*args, st, dt_bias=g["dt_bias"])
+        assert torch.equal(st, before)
+        g["dt"][:, 66] = float("nan")
+        y, fin = gdn_hip.ssm_scan(g["x"], g["dt"], g["A_log"], g["B"], g["C"], g["D"], g["z"], g["dt_bias"])
+        torch.cuda.synchronize()
+        assert torch.isfinite(y[:, :66]).all() and torch.isnan(y[:, 66:]).all() and torch.isnan(fin).all()
+
+
+def test_fp16_extreme_scales(dev):
+    """fp16 inputs at both ends of the type, steps up to 1e4: the scales in
+    front of the products keep every part in range."""
+    for fx, fb, fc, lift in ((2000.0, 100.0, 5e-6, 0.0), (1e-4, 1e-3, 1e3, -8.0), (1e-3, 1.0, 1.0, 9.2)):
+        d = sc.inputs(31, 1, 140, 2, 64, 1, 64, HF, dt_dtype=torch.float32)
+        d["x"], d["B"], d["C"] = d["x"] * fx, d["B"] * fb, d["C"] * fc
+        assert all(torch.isfinite(d[k]).all() for k in "xBC")
+        d["dt_bias"] = d["dt_bias"] + lift if lift < 9 else d["dt_bias"] + 10.0 ** 4
+        d["D"] = d["D"] / fx
+        _check_scan(dev, d, None, HF, f"fp16 scales x {fx} B {fb} step {lift}")
+
+
 def test_scan_rows_behind_the_last_sequence(dev):
     """C entry: y rows behind the last packed sequence are left as they were."""
     import ctypes as ct
@@ -166,8 +249,8 @@ def test_step_slots(dev):
     rest = [d[k] for k in ("D", "z", "dt_bias")]
     pool = _s0(6, 9, 4, 128, 64).to(dev)
     before = pool.clone()
-    slots = [7, -1, 0, 9, 3]   # 9: past the pool
-    for dt in (torch.int32, torch.int64):
+    for dt, past in ((torch.int32, 9), (torch.int64, 9), (torch.int64, 2 ** 32 + 1)):
+        slots = [7, -1, 0, past, 3]
         pool.copy_(before)
         y = gdn_hip.ssm_step(*args, pool, *rest, slots=torch.tensor(slots, dtype=dt, device=dev))
         live = [0, 2, 4]

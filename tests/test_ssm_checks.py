@@ -23,7 +23,8 @@ def _inputs(**over):
 
 
 BAD = [dict(x=None), dict(dt=None), dict(b=None), dict(c=None), dict(A_log=None), dict(x=P + 8),
-       dict(z=P + 2), dict(b=P + 4), dict(x_token=12), dict(c_token=-8), dict(b_token=1 << 31),
+       dict(z=P + 2), dict(b=P + 4), dict(x_token=12), dict(c_token=-8), dict(b_token=1 << 24),
+       dict(x_token=1 << 24), dict(heads=1 << 18, groups=2),
        dict(dt_token=-1), dict(z_batch=4), dict(batch=0), dict(tokens=-1), dict(heads=0),
        dict(groups=3), dict(groups=0), dict(head_dim=8), dict(head_dim=72), dict(head_dim=272),
        dict(state_dim=48), dict(state_dim=512), dict(io_dtype=2), dict(dt_dtype=1),
@@ -34,7 +35,7 @@ BAD = [dict(x=None), dict(dt=None), dict(b=None), dict(c=None), dict(A_log=None)
 def test_ssm_refuses(bad):
     lib, a = capi.lib(), _inputs(**bad)
     assert lib.gdn_ssm_step(ct.byref(a), P, P, None, 0, None) == INVALID
-    assert lib.gdn_ssm_scan(ct.byref(a), P, P, P, None, None, a.batch, 64, P, 1 << 40, None) == INVALID
+    assert lib.gdn_ssm_scan(ct.byref(a), P, P, 2 * P, None, None, a.batch, 64, P, 1 << 40, None) == INVALID
 
 
 def test_ssm_refuses_outputs_and_tables():
@@ -46,7 +47,8 @@ def test_ssm_refuses_outputs_and_tables():
     assert lib.gdn_ssm_step(None, P, P, None, 0, None) == INVALID
     need = lib.gdn_ssm_scan_workspace_size(r, 2, 64, 0)
     assert need > 0
-    ok = [r, P, P, P, None, None, 2, 64, P, need, None]
+    ok = [r, P, P, 2 * P, None, None, 2, 64, P, need, None]
+    assert lib.gdn_ssm_scan(r, P, P, P, None, None, 2, 64, P, need, None) == INVALID   # sf is s0
 
     def scan(**over):
         args = list(ok)
