@@ -16,7 +16,9 @@
 // lengths to the last store.  Up to kOneLaunch requests every work-group
 // forms both prefix sums of the whole batch for itself in LDS and then fills
 // its own part of the tables; past that a single group writes them and a
-// second launch searches them in the cache.
+// second launch searches them in the cache.  4.2 us for 8 requests, 8.2 for
+// 1500 with 274,000 tokens (12 with a scan per 256 requests in place of a
+// thread's run of requests and one scan).
 #include "gdn_common.h"
 #include "gdn_hip.h"
 

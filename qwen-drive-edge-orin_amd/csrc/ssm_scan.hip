@@ -14,17 +14,36 @@
 // of the segments, and the main pass starts each segment from its own.  A
 // call whose sequences have one segment each runs the main pass alone.
 //
-// A wave owns 16 PT columns of one head: its slice of S stays in fp32
-// accumulators through the segment, and the columns need nothing from one
-// another.  Four waves of one group share B, C and the products C B^T in LDS.
+// A wave owns 32 columns of one head: its slice of S stays in fp32 accumulators
+// through the segment, and the columns need nothing from one another.  Four
+// waves of one group share B, C and the products C B^T in LDS, 80 KB a
+// work-group (state 128), so that two groups fit a CU and their 2 waves a SIMD
+// cover each other's waits; 64 columns a wave would save a fifth of the vector
+// work (M is formed once per wave) but hold 128 registers of S more and leave
+// one wave a SIMD (measured at an early stage: 693 us against 398 for the
+// packed call below).  The next chunk's tiles go into LDS while the present
+// one is worked on.
 // The MFMA operand and result layouts (gdn_common.h) chain without shuffles:
 // S's tiles are the A operand of S^T C^T, C B^T comes out transposed as the B
 // operand of X^T M^T, and rows are numbered so that two result tiles hold 8
 // consecutive channels (perm below), 16 bytes of y.
 //
+// Measured (state 128): 8 packed prompts, 19,861 tokens x 64 heads of 64 with
+// the gate: 299 us, 2.0 TB/s of what must move: main pass 220, first pass 81,
+// join 15, table 3.  16,384 tokens x 16 heads 74 us, 1141 x 64 37 us.  In the
+// main pass the SIMDs issue vector instructions 49 % of the time and the MFMA
+// units are busy 26 % (0.6 PFLOP/s): two waves a SIMD, each in order, with a
+// seventh of the products for operands' second and third parts and M's
+// exponentials, splits and the gate on the vector units.  Measured without
+// gain: waves' priorities raised in the MFMA or the vector phases, update and M
+// interleaved by quarters of the chunk (spills), 8-wave groups, operand
+// residuals by dot products.
+//
 // Rounding.  bf16: x, B and C are exact operands; S and M = (C B^T) o decay
-// enter y's products as pairs of bf16 (2^-17 of each term, y itself has 2^-8),
-// and d x, which enters the state, as three (2^-25).  Sums, states, decays:
+// enter y's products as pairs of bf16 (2^-18 of each term, y itself has 2^-8),
+// and d x, which enters the state, as three (fp32's 24 bits; two would leave
+// 2.4e-6 of the state).  fp16: pairs of fp16 behind a power-of-two scale that
+// fits them (22 bits).  Sums, states, decays:
 // fp32.  Logarithms are summed in fp32 forwards for c and backwards for the
 // state's weights, so that the weights of the newest tokens, the largest, are
 // sums of few terms; a token's base-2 logarithm is held at -150, where its
@@ -41,8 +60,8 @@ namespace {
 constexpr int kMaxBlock = 1 << 20;
 // Segments of a fixed-length sequence that the main pass joins by itself: each
 // group reads the records in front of its own, which is less than a launch of
-// the join up to here (1141 tokens x 64 heads in 6
-// segments: 38 us against 41; 4 x 2048 tokens x 32 in 8: 95 against 82)
+// the join up to here (1141 tokens x 64 heads in 6 segments: 38 us against 41;
+// 4 x 2048 tokens x 32 in 8: 95 against 82)
 constexpr int kMaxFold = 6;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
