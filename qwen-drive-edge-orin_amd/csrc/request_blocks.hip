@@ -34,7 +34,7 @@ constexpr int kTokens = 4;                  // consecutive tokens a thread fills
 constexpr int kScanThreads = 1024;          // the single group of the two-launch form
 
 __device__ __forceinline__ int sat(int a, int b, int top) {   // 0 <= a, b <= top <= 2^30
-    return min(a + b, top);
+    return (int)min((uint32_t)a + (uint32_t)b, (uint32_t)top);   // (2^30 + 2^30 passes an int)
 }
 
 __device__ __forceinline__ int rows_of(int n, int block) { return max(1, (n + block - 1) / block); }

@@ -343,3 +343,77 @@ def test_other_stream(dev):
     s.synchronize()
     for a, b in zip(ref, got):
         assert torch.equal(a, b)
+
+
+def test_request_blocks_largest(dev):
+    """2^30 tokens, and lengths that pass them twice over."""
+    total, block = 1 << 30, 1 << 20
+    for lengths in ([2 ** 31 - 1, 2 ** 31 - 1, 5], [0, 2 ** 30, 2 ** 30]):
+        print(f"request_blocks {lengths} in {total}", flush=True)
+        cu, table, slot, pos = gdn_hip.request_blocks(
+            torch.tensor(lengths, dtype=torch.int32, device=dev), total, block=block)
+        torch.cuda.synchronize()
+        full = lengths.index(max(lengths))
+        assert cu.tolist() == [0] * (full + 1) + [total] * (3 - full)
+        rows = [[n, 0, 0, 0] for n in range(full)] + \
+            [[full, i * block, block, i] for i in range(total // block)] + \
+            [[n, total, 0, 0] for n in range(full + 1, 3)]
+        assert table.tolist() == rows + [[-1, 0, 0, 0]] * (table.shape[0] - len(rows))
+        assert (slot == full).all() and torch.equal(pos, torch.arange(total, dtype=torch.int32, device=dev))
+
+
+def test_conv_and_norm_offsets_past_32_bits(dev):
+    T, D = 540_700, 4096   # 2.2e9 elements
+    x = torch.randn(1, T, D, device=dev, dtype=BF)
+    w = (0.5 * torch.randn(D, 4, generator=torch.Generator().manual_seed(1))).to(BF)
+    tail = x[:, -40:].cpu().transpose(1, 2)
+    for cu in (None, torch.tensor([0, T - 9, T], dtype=torch.int32, device=dev)):
+        print(f"conv over {T} x {D}, packed {cu is not None}", flush=True)
+        y, st = gdn_hip.causal_conv1d_prefill(x.transpose(1, 2), w.to(dev), silu=True, cu_seqlens=cu)
+        torch.cuda.synchronize()
+        ref, rst, mag = orc.conv_prefill(tail, w, None, None, True, None if cu is None else [31, 9])
+        sc.close(y[:, :, -36:], ref[:, :, 4:], _conv_bound(ref, mag, BF, True)[:, :, 4:], "conv tail")
+        assert torch.equal(st[-1:].double().cpu(), rst[-1:])
+    print(f"norm of {T} x {D}", flush=True)
+    y = gdn_hip.gated_groupnorm(x[0], x[0], w[:, 0].contiguous().to(dev), 2)
+    torch.cuda.synchronize()
+    last = x[0, -5:].cpu()
+    ref = orc.gated_groupnorm(last, last, w[:, 0], 2, 1e-6)
+    half = 2.0 ** -8
+    sc.close(y[-5:], ref, (half + 2.0 ** -18) * ref.abs() + torch.finfo(BF).smallest_normal * half, "norm tail")
+
+
+def test_conv_rows_behind_the_last_sequence(dev):
+    """C entry: y rows behind the last packed sequence are left as they were."""
+    from gdn_hip import capi
+    x, w, _, s0 = _conv_inputs(8, 1, 100, 64, 4, 4, BF, BF, 3)
+    xd, wd, sd = x.transpose(1, 2).contiguous().to(dev), w.to(dev), s0.to(dev)
+    y = torch.full((1, 100, 64), 7.0, dtype=BF, device=dev)
+    st = torch.empty_like(sd)
+    cu = torch.tensor([0, 30, 30, 71], dtype=torch.int32, device=dev)
+    assert capi.lib().gdn_causal_conv1d_prefill(
+        xd.data_ptr(), wd.data_ptr(), None, sd.data_ptr(), y.data_ptr(), st.data_ptr(), 1, 100, 64, 4, 4,
+        6400, 64, 6400, 64, cu.data_ptr(), 3, 0, 0, 1, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    ref, rst, mag = orc.conv_prefill(x, w, None, s0, True, [30, 0, 41])
+    sc.close(y[:, :71].transpose(1, 2), ref, _conv_bound(ref, mag, BF, True), "conv in front")
+    assert (y[:, 71:] == 7).all() and torch.equal(st.double().cpu(), rst)
+
+
+def test_two_streams_at_once(dev):
+    """Two prompts batches on two streams, neither waiting for the other."""
+    layer = _Layer(dev)
+    ins = [_layer_inputs(layer, lengths, seed) for lengths, seed in (([700, 3], 4), ([300, 400], 5))]
+    refs = [layer.prompts(*i, None, None) for i in ins]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(4):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(layer.prompts(*ins[k], None, None))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for out in got[k]:
+            for a, b in zip(refs[k], out):
+                assert torch.equal(a, b)
