@@ -388,7 +388,8 @@ hipError_t gdn_gated_groupnorm_forward(const void* x, int64_t x_row, const void*
 
 /* gdn_causal_conv1d_update on a pool of num_slots conv states: row b uses
  * state slots[b] (device int32 [B]); a slot outside the pool is a row without
- * a request: its y is zero and no state changes. */
+ * a request: its y is zero and no state changes.  Two rows of a call must not
+ * name one slot (their results would be undefined, in bounds). */
 hipError_t gdn_causal_conv1d_update_slots(const void* x, void* conv_state, const void* w,
                                           const void* bias, void* y, const int32_t* slots,
                                           int num_slots, int B, int T, int D, int K,

@@ -580,6 +580,9 @@ at::Tensor causal_conv1d_update_slots(const at::Tensor& x, at::Tensor conv_state
                     (!bias || bias->is_cuda()),
                 "all inputs must be CUDA tensors");
     TORCH_CHECK(x.dim() == 3, "x must be [B, D, T]");
+    TORCH_CHECK(conv_state.device() == x.device() && weight.device() == x.device() &&
+                    (!bias || bias->device() == x.device()),
+                "all inputs must be on x's device");
     const int64_t B = x.size(0), D = x.size(1), T = x.size(2);
     TORCH_CHECK(conv_state.dim() == 3 && conv_state.size(1) == D && conv_state.size(0) >= 1 &&
                     conv_state.size(0) <= 0x7fffffff,
