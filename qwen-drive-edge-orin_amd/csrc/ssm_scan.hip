@@ -44,10 +44,11 @@
 // and d x, which enters the state, as three (fp32's 24 bits; two would leave
 // 2.4e-6 of the state).  fp16: pairs of fp16 behind a power-of-two scale that
 // fits them (22 bits).  Sums, states, decays:
-// fp32.  Logarithms are summed in fp32 forwards for c and backwards for the
-// state's weights, so that the weights of the newest tokens, the largest, are
-// sums of few terms; a token's base-2 logarithm is held at -150, where its
-// decay is 0 in fp32, to keep differences of c exact for the tokens behind it.
+// fp32.  Logarithms are summed in fp32, forwards within 16 tokens for M and
+// backwards for the state's weights, so that the weights of the newest tokens,
+// the largest, are sums of few terms; a token's base-2 logarithm is held at
+// -150, where its decay is 0 in fp32, to keep the differences of M exact for
+// the tokens behind it.
 #include "gdn_seq.h"
 #include "gdn_ssm.h"
 
@@ -233,19 +234,31 @@ struct Stager {
     }
 };
 
-// Inclusive sums over lanes 0 .. lane (DPP: within rows of 16, then across)
-__device__ __forceinline__ float lane_prefix(float x) {
-#define GDN_DPP(ctrl, rows)                                                                      \
-    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(                                  \
-                                       0, __builtin_bit_cast(int, x), ctrl, rows, 0xf, false))
-    GDN_DPP(0x111, 0xf);   // row_shr:1
-    GDN_DPP(0x112, 0xf);
-    GDN_DPP(0x114, 0xf);
-    GDN_DPP(0x118, 0xf);
-    GDN_DPP(0x142, 0xa);   // row_bcast:15 into rows 1 and 3
-    GDN_DPP(0x143, 0xc);   // row_bcast:31 into rows 2 and 3
+// Inclusive sums within a row of 16 lanes: over the lanes up to this one
+__device__ __forceinline__ float row_prefix(float x) {
+#define GDN_DPP(ctrl)                                                                             \
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(                                   \
+                                       0, __builtin_bit_cast(int, x), ctrl, 0xf, 0xf, false))
+    GDN_DPP(0x111);   // row_shr:1
+    GDN_DPP(0x112);
+    GDN_DPP(0x114);
+    GDN_DPP(0x118);
+    return x;
+}
+
+// and over this one and the lanes behind it
+__device__ __forceinline__ float row_suffix(float x) {
+    GDN_DPP(0x101);   // row_shl:1
+    GDN_DPP(0x102);
+    GDN_DPP(0x104);
+    GDN_DPP(0x108);
 #undef GDN_DPP
     return x;
+}
+
+// x of the next lane of the row, 0 for its last
+__device__ __forceinline__ float row_next(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x101, 0xf, 0xf, false));
 }
 
 // The largest of non-negative x over the wave
@@ -281,10 +294,11 @@ struct Smem {
     uint16_t c[kLocal ? 8 : 64 * N];
     uint16_t x[WAVES][64 * 16 * PT];
     f32x4 cb[kLocal ? 1 : 10][64];   // (C B^T)^T tiles of the lower triangle, as fragments
-    // per token of the chunk, for each wave's head: c; the step d; the weight
-    // in S; d e^{c_ref - c}, c_ref the last c of the token's 16
+    // per token of the chunk, for each wave's head: the sum r of the log decays
+    // of its 16 up to it; the step d; the weight in S; d times the decay up to
+    // the end of its 16
     struct {
-        float c2[64], d[64], w[64], f[64];
+        float r[64], d[64], w[64], f[64];
     } tok[WAVES];
 };
 
@@ -405,24 +419,31 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
     int kappa = 0;
     float d_max = 0.f, w_max = 0.f;
 
-    // Token `lane` of a chunk of n: step, log decay, its sums from the chunk's
-    // start and from its end
+    // Token `lane` of a chunk of n: step, log decay, its sums.  They are kept
+    // by 16 tokens, with the sums of whole 16s apart: where strong decays
+    // (resets) and weak ones alternate, the difference of two sums over a whole
+    // chunk loses up to 7e-4 of a decay, that of two sums within 16 tokens 2e-4.
+    float sums[4];
     auto token_vectors = [&](float raw, int n) {
         const float d = lane < n ? ssm_delta(raw, bias, in.dt_min, in.dt_max) : 0.f;
         const float l2 = lane < n ? fmaxf(A2 * d, -150.f) : 0.f;
-        const float c2 = lane_prefix(l2);
-        // lane i of the reversed order is token 63 - i
-        const float back = lane_prefix(__shfl(l2, 63 - lane, 64));
-        const float after = __shfl(back, 62 - lane, 64);   // tokens lane + 1 ..
-        tok.c2[lane] = c2;
-        tok.d[lane] = d;
-        const float w = d * __builtin_amdgcn_exp2f(lane < 63 ? after : 0.f);
+        const float from = row_suffix(l2);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            sums[k] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, from), 16 * k));
+        const float after = row_next(from);
+        const float behind = g == 0 ? sums[1] + (sums[2] + sums[3]) : g == 1 ? sums[2] + sums[3] : g == 2 ? sums[3] : 0.f;
+        const float w = d * __builtin_amdgcn_exp2f(after + behind);
         tok.w[lane] = w;
         if (IO == 1) {
             d_max = wave_max(d);
             w_max = wave_max(w);
         }
-        if (!kLocal) tok.f[lane] = d * __builtin_amdgcn_exp2f(__shfl(c2, lane | 15, 64) - c2);
+        if (!kLocal) {
+            tok.r[lane] = row_prefix(l2);
+            tok.d[lane] = d;
+            tok.f[lane] = d * __builtin_amdgcn_exp2f(after);
+        }
     };
 
     f32x4 Dd;   // D on the diagonal of a tile
@@ -558,8 +579,10 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
             float ct[4];
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt) {
-                ct[tt] = tok.c2[16 * tt + m];
-                const float e = __builtin_amdgcn_exp2f(IO == 1 ? ct[tt] + (float)(k_m - k_s - kappa) : ct[tt]);
+                ct[tt] = tok.r[16 * tt + m];
+                const float before = tt == 0 ? 0.f : tt == 1 ? sums[0] : tt == 2 ? sums[0] + sums[1] : sums[0] + (sums[1] + sums[2]);
+                const float c = ct[tt] + before;
+                const float e = __builtin_amdgcn_exp2f(IO == 1 ? c + (float)(k_m - k_s - kappa) : c);
                 if (IO == 1) ct[tt] += (float)k_m;
 #pragma unroll
                 for (int pt = 0; pt < PT; ++pt) Y[pt][tt] *= e;
@@ -580,17 +603,18 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
                             for (int i = 0; i < 4; ++i) v[4 * q + i] = 0.f;
                         } else if (st == tt) {
                             const f32x4 cb = sm.cb[tri(tt, st)][lane];
-                            const f32x4 cs = *reinterpret_cast<const f32x4*>(tok.c2 + 16 * st + 4 * g);
+                            const f32x4 rs = *reinterpret_cast<const f32x4*>(tok.r + 16 * st + 4 * g);
                             const f32x4 ds = *reinterpret_cast<const f32x4*>(tok.d + 16 * st + 4 * g);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const float e = cb[i] * __builtin_amdgcn_exp2f(ct[tt] - cs[i]) * ds[i];
+                                const float e = cb[i] * __builtin_amdgcn_exp2f(ct[tt] - rs[i]) * ds[i];
                                 v[4 * q + i] = (4 * g + i <= m ? e : 0.f) + Dm[i];
                             }
                         } else {
                             const f32x4 cb = sm.cb[tri(tt, st)][lane];
                             const f32x4 fs = *reinterpret_cast<const f32x4*>(tok.f + 16 * st + 4 * g);
-                            const float ht = __builtin_amdgcn_exp2f(ct[tt] - tok.c2[16 * st + 15]);
+                            const float between = tt - st == 1 ? 0.f : tt - st == 2 ? sums[st + 1] : sums[1] + sums[2];
+                            const float ht = __builtin_amdgcn_exp2f(ct[tt] + between);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) v[4 * q + i] = cb[i] * (fs[i] * ht);
                         }
@@ -637,7 +661,7 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
         }
 
         // S <- e^{c_Q} S + B^T (w x)
-        const float total2 = tok.c2[63];
+        const float total2 = (sums[0] + sums[1]) + (sums[2] + sums[3]);
         float dec = __builtin_amdgcn_exp2f(total2), w_scale = 1.f;
         log_total += total2;
         if constexpr (IO == 1) {
@@ -969,9 +993,9 @@ static double passes_us(double groups, double chunks, int deep, const double* t,
 // to 64 KB a record and pass).  The constants are measured at state_dim 128
 // (main pass: 5.7 and 8.8 us a chunk with one and two groups on a CU; first pass
 // 2.9, 3.3 and 3.6 with one to three; about 5 us to start a group from its
-// state), the rule's choices at most 16 % slower than the best of 1 .. 256
-// chunks over 19 calls (77 to 65,536 tokens, 8 to 128 heads, 1 to 101 sequences),
-// 3 % on average.
+// state), the rule's choices at most 11 % slower than the best of 1 .. 256
+// chunks over 23 calls (77 to 65,536 tokens, 8 to 128 heads, 1 to 101 sequences),
+// 2 % on average.
 extern "C" int gdn_ssm_scan_block(const gdn_ssm_inputs* in, int num_seqs) {
     if (!ssm_sizes_ok(in) || num_seqs < 1 || in->tokens > (1 << 30)) return 0;
     const int tasks = in->heads / in->groups * ((in->head_dim + kCols - 1) / kCols);

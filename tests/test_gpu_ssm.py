@@ -72,6 +72,30 @@ def test_scan_reset_token(dev):
     _check_scan(dev, d, _s0(9, 1, 2, 128, 64), BF, "scan reset")
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_scan_resets_and_weak_decays(dev, dtype):
+    """Every other token or so wipes the state, the others hardly decay it.
+
+    The weight of one of 16 tokens for another of them is a difference of two
+    sums of base-2 log decays, each held at -150 or above: sums of 2, 4, 8 and
+    16 tokens below 512, 1024, 2048 and 4096 in magnitude are off by up to
+    2^-16, 2^-15, 2^-14 and 2^-13, so the difference by 2 (15/8) 2^-13 and the
+    weight by that times ln 2, relative: below 2^-11.5.  Sums of whole 16s keep
+    the sign, and count only where they are no reset."""
+    d = sc.inputs(21, 1, 330, 3, 64, 1, 128, dtype, dt_dtype=torch.float32)
+    wipe = torch.rand(330, generator=torch.Generator().manual_seed(5)) < 0.5
+    d["dt"] = torch.where(wipe[None, :, None], torch.tensor(1e4), d["dt"] - 2)
+    d["x"] = torch.where(wipe[None, :, None, None], torch.zeros((), dtype=dtype), d["x"])
+    s0 = _s0(4, 1, 3, 128, 64)
+    y, S, ya, Sa = orc.ssm(d["x"], d["dt"], d["A_log"], d["B"], d["C"], d["D"], d["z"], d["dt_bias"], s0)
+    g = sc.to(d, dev)
+    oy, oS = gdn_hip.ssm_scan(g["x"], g["dt"], g["A_log"], g["B"], g["C"], g["D"], g["z"], g["dt_bias"], s0.to(dev))
+    torch.cuda.synchronize()
+    by, bS = sc.bounds(d, 330, y, ya, Sa, dtype)
+    sc.close(oy, y, by + 2.0 ** -11.5 * ya, f"resets {dtype} y")
+    sc.close(oS, S, bS, f"resets {dtype} state")
+
+
 def test_scan_large_and_small_values(dev):
     """bf16 values far outside 16-bit floats of five exponent bits."""
     for f in (1e10, 1e-10):
@@ -262,6 +286,46 @@ def test_step_slots(dev):
         assert torch.equal(pool[[7, 0, 3]], st)
         keep = [i for i in range(9) if i not in (7, 0, 3)]
         assert torch.equal(pool[keep], before[keep])
+
+
+def test_scan_offsets_past_32_bits(dev):
+    """2.2e9 elements of x: the last tokens against the recurrence from some way
+    in front (a token decays by e^-0.7 on average, 100 of them to nothing)."""
+    T, H = 540_700, 64
+    x = torch.randn(1, T, H, 64, device=dev, dtype=BF)
+    b, c = (torch.randn(1, T, 1, 64, device=dev, dtype=BF) for _ in range(2))
+    dt = torch.randn(1, T, H, device=dev, dtype=BF)
+    d = dict(x=x, dt=dt, A_log=torch.zeros(H, device=dev), B=b, C=c, D=None, z=x,
+             dt_bias=torch.zeros(H, device=dev))
+    n = 160
+    cut = {k: (v if k in ("A_log", "dt_bias") else None if v is None else v[:, -n:]) for k, v in d.items()}
+    cut = {k: None if v is None else v.cpu() for k, v in cut.items()}
+    y, S, ya, Sa = orc.ssm(**cut)
+    by, bS = sc.bounds(cut, n, y, ya, Sa, BF)
+    for cu in (None, torch.tensor([0, T - n, T], dtype=torch.int32, device=dev)):
+        print(f"scan over {T} tokens, packed {cu is not None}", flush=True)
+        oy, oS = gdn_hip.ssm_scan(**d, cu_seqlens=cu)
+        torch.cuda.synchronize()
+        lo = 0 if cu is not None else 120
+        sc.close(oy[:, T - n + lo:], y[:, lo:], by[:, lo:], "scan tail y")
+        sc.close(oS[-1:], S, bS, "scan tail state")
+
+
+def test_step_pool_past_32_bits(dev):
+    """A pool of 4200 states of 2 MB: 2.2e9 elements."""
+    pool = torch.zeros(4200, 64, 128, 64, device=dev)
+    d = sc.inputs(3, 2, 1, 64, 64, 1, 128)
+    y, S, ya, Sa = orc.ssm(**d)
+    g = sc.to(d, dev)
+    print("step, slots 4199 and 4100", flush=True)
+    oy = gdn_hip.ssm_step(g["x"], g["dt"], g["A_log"], g["B"], g["C"], pool, g["D"], g["z"], g["dt_bias"],
+                          slots=torch.tensor([4199, 4100], dtype=torch.int32, device=dev))
+    torch.cuda.synchronize()
+    by, bS = sc.bounds(d, 1, y, ya, Sa, BF)
+    sc.close(oy, y, by, "step y")
+    sc.close(pool[[4199, 4100]], S, bS, "step states")
+    pool[[4199, 4100]] = 0
+    assert not pool.any()
 
 
 def test_no_tokens(dev):
