@@ -1047,7 +1047,7 @@ extern "C" hipError_t gdn_ssm_scan(const gdn_ssm_inputs* in, void* y, const floa
     const bool packed = cu_seqlens != nullptr;
     if (!ssm_inputs_ok(in) || !scan_sizes_ok(in, num_seqs, block, packed) || (blocks && !packed))
         return hipErrorInvalidValue;
-    if (!sf || sf == s0 || !ssm_aligned(sf, 4) || !ssm_aligned(s0, 4) || (in->tokens > 0 && !y) ||
+    if (!in->A_log || !sf || sf == s0 || !ssm_aligned(sf, 4) || !ssm_aligned(s0, 4) || (in->tokens > 0 && !y) ||
         !ssm_aligned(y, 16) || !ssm_aligned(workspace, 256) || !ssm_aligned(blocks, 16))
         return hipErrorInvalidValue;
     const size_t need = gdn_ssm_scan_workspace_size(in, num_seqs, block, packed);

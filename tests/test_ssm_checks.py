@@ -69,6 +69,14 @@ def test_ssm_refuses_outputs_and_tables():
     assert lib.gdn_ssm_scan_block(r, 2) % 64 == 0 and lib.gdn_ssm_scan_block(r, 2) >= 64
 
 
+def test_scan_without_tokens_still_needs_a_log():
+    """States pass through such a call, and its kernels read A_log."""
+    lib = capi.lib()
+    for state_dim in (16, 128):
+        a = _inputs(tokens=0, A_log=None, state_dim=state_dim)
+        assert lib.gdn_ssm_scan(ct.byref(a), P, P, 2 * P, None, None, 2, 64, P, 1 << 40, None) == INVALID
+
+
 def test_workspace_covers_every_split():
     """The packed bound holds for any lengths, empty sequences too."""
     lib = capi.lib()
