@@ -29,7 +29,7 @@
 // consecutive channels (perm below), 16 bytes of y.
 //
 // Measured (state 128): 8 packed prompts, 19,861 tokens x 64 heads of 64 with
-// the gate: 299 us, 2.0 TB/s of what must move: main pass 220, first pass 81,
+// the gate: 296 us, 2.0 TB/s of what must move: main pass 220, first pass 81,
 // join 15, table 3.  16,384 tokens x 16 heads 74 us, 1141 x 64 37 us.  In the
 // main pass the SIMDs issue vector instructions 49 % of the time and the MFMA
 // units are busy 26 % (0.6 PFLOP/s): two waves a SIMD, each in order, with a
@@ -64,6 +64,10 @@ constexpr int kMaxBlock = 1 << 20;
 // the join up to here (1141 tokens x 64 heads in 6 segments: 38 us against 41;
 // 4 x 2048 tokens x 32 in 8: 95 against 82)
 constexpr int kMaxFold = 6;
+// Work-groups of a packed call up to which the main pass takes the longest
+// segments first (8 rounds of 512: what the last round wastes still counts
+// against a group's one more trip to memory)
+constexpr int kMaxOrder = 4096;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kTiles = 2;          // 16-column tiles of a wave
@@ -87,6 +91,7 @@ struct ScanArgs {
     int tasks;           // slices of a group: heads / groups x slices
     bool fold;           // the main pass joins the segments' states itself
     int quads;           // work-groups per group and segment: ceil(tasks / waves)
+    int* order;          // the main pass's rows, longest first; null: as they lie
     f32x4* states;       // [row][group][task] fragments of a slice's state
     float* decays;       // [row][group][task]
 };
@@ -304,6 +309,23 @@ struct Smem {
 
 __device__ __forceinline__ constexpr int tri(int tt, int st) { return tt * (tt + 1) / 2 + st; }
 
+// Row r's place in the main pass, by a whole group: the longest segments first,
+// so that what ends last is short.  Places are unique whatever the table holds.
+__device__ __forceinline__ void order_row(const ScanArgs& a, int r) {
+    __shared__ int count[kWaves];
+    const int n = a.table[r].z;
+    int before = 0;
+    for (int j = threadIdx.x; j < a.rows; j += kThreads) {
+        const int m = a.table[j].z;
+        before += m > n || (m == n && j < r);
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) before += __shfl_xor(before, off, 64);
+    if ((threadIdx.x & 63) == 0) count[threadIdx.x >> 6] = before;
+    __syncthreads();
+    if (threadIdx.x == 0) a.order[count[0] + count[1] + count[2] + count[3]] = r;
+}
+
 // kLocal: the first pass (states only)
 template <int IO, int N, int PT, int WAVES, bool kLocal>
 __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(const ScanArgs a) {
@@ -320,7 +342,12 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
     // are dealt over all of them, so that short ones even out.
     const int xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
     const int quad = nth % a.quads, unit = nth / a.quads * 8 + xcd;
-    const int grp = unit % in.groups, row = unit / in.groups;
+    const int grp = unit % in.groups;
+    int row = unit / in.groups;
+    if (a.order && row < a.rows) {
+        if (!kLocal) row = a.order[row];
+        else if (grp == 0 && quad == 0) order_row(a, row);
+    }
     Seg s;
     if (row >= a.rows || !segment(a, row, s) || (kLocal && s.last)) return;
     const int task = quad * WAVES + wave;
@@ -896,7 +923,8 @@ struct Layout {
     int segs;        // segments of a batch row (0: packed)
     int64_t rows;
     int slices, tasks, quads;
-    size_t table, starts, states, decays, total;   // byte offsets
+    bool ordered;
+    size_t table, starts, order, states, decays, total;   // byte offsets
 
     Layout(const gdn_ssm_inputs* in, int seqs, int block, bool packed) {
         segs = packed ? 0 : std::max(1, (in->tokens + block - 1) / block);
@@ -909,6 +937,9 @@ struct Layout {
         if (packed) off += align256((size_t)rows * 16);
         starts = off;
         if (packed) off += align256(((size_t)seqs + 1) * 4);
+        order = off;
+        ordered = packed && rows * in->groups * quads <= kMaxOrder;
+        if (ordered) off += align256((size_t)rows * 4);
         // no states where every sequence is one segment
         const size_t recs = packed || segs > 1 ? (size_t)rows * in->groups * tasks : 0;
         states = off;
@@ -996,6 +1027,14 @@ static double passes_us(double groups, double chunks, int deep, const double* t,
 // state), the rule's choices at most 11 % slower than the best of 1 .. 256
 // chunks over 23 calls (77 to 65,536 tokens, 8 to 128 heads, 1 to 101 sequences),
 // 2 % on average.
+//
+// A packed batch whose sequences fill the chip 1.2 times without a split is
+// split only where one would hold the others up: at 1.5 times the chunks that
+// a place then works off (30 prompts of 50 to 2000 tokens x 64 heads: 331 us
+// against 442 by the estimate above).  The lengths are on the GPU, so what a
+// packed call takes is a guess: over 192 batches (2 to 64 prompts, uniform
+// lengths, and one long among short ones) the choices are 4 % slower on average
+// than the best, at most 37 %.
 extern "C" int gdn_ssm_scan_block(const gdn_ssm_inputs* in, int num_seqs) {
     if (!ssm_sizes_ok(in) || num_seqs < 1 || in->tokens > (1 << 30)) return 0;
     const int tasks = in->heads / in->groups * ((in->head_dim + kCols - 1) / kCols);
@@ -1007,10 +1046,15 @@ extern "C" int gdn_ssm_scan_block(const gdn_ssm_inputs* in, int num_seqs) {
     // a group's chunks: packed sequences differ, the longest of a few is about
     // 1.7 times the average
     const double longest = packed ? 1.7 * per_seq : per_seq;
+    const int deep = in->state_dim == 256 ? 1 : 2, local_deep = in->state_dim == 256 ? 1 : 3;
+    const double places = 256.0 * deep;
+    if (packed && num_seqs * units >= 1.2 * places) {
+        const double each = ((double)in->tokens / kChunk + 0.5 * num_seqs) * units / places;
+        return (int)std::min(std::ceil(1.5 * each), (double)(kMaxBlock / kChunk)) * kChunk;
+    }
     const double main_t[2] = {5.7, 8.8}, local_t[3] = {2.9, 3.3, 3.6};
     const double record_us = (double)in->groups * tasks * in->state_dim * kCols * 4 / 5e6;
     const double scale = in->state_dim / 128.0;
-    const int deep = in->state_dim == 256 ? 1 : 2, local_deep = in->state_dim == 256 ? 1 : 3;
     int best = 1;
     double least = 0;
     for (int c = 1; c <= kMaxBlock / kChunk; c += c < 16 ? 1 : c / 8) {
@@ -1071,6 +1115,7 @@ extern "C" hipError_t gdn_ssm_scan(const gdn_ssm_inputs* in, void* y, const floa
     a.states = reinterpret_cast<f32x4*>(ws + l.states);
     a.decays = reinterpret_cast<float*>(ws + l.decays);
     if (packed) {
+        if (l.ordered) a.order = reinterpret_cast<int*>(ws + l.order);
         a.table = reinterpret_cast<const int4*>(blocks);
         if (!blocks) {
             auto table = reinterpret_cast<int4*>(ws + l.table);

@@ -77,6 +77,18 @@ def test_scan_without_tokens_still_needs_a_log():
         assert lib.gdn_ssm_scan(ct.byref(a), P, P, 2 * P, None, None, 2, 64, P, 1 << 40, None) == INVALID
 
 
+@pytest.mark.parametrize("tokens", [0, 1, 1000, 1 << 17, 1 << 30])
+def test_block_is_one_the_scan_takes(tokens):
+    """Blocks and workspaces for one sequence, many, and more than fill the chip."""
+    lib = capi.lib()
+    for seqs in (1, 2, 40, 3000):
+        for heads, state_dim in ((2, 32), (64, 128), (64, 256)):
+            a = _inputs(batch=1, tokens=tokens, heads=heads, state_dim=state_dim)
+            block = lib.gdn_ssm_scan_block(ct.byref(a), seqs)
+            assert 64 <= block <= 1 << 20 and block % 64 == 0
+            assert lib.gdn_ssm_scan_workspace_size(ct.byref(a), seqs, block, 1) > 0
+
+
 def test_workspace_covers_every_split():
     """The packed bound holds for any lengths, empty sequences too."""
     lib = capi.lib()
