@@ -222,18 +222,13 @@ def _own(s):
                                gate_first=s["gate_first"])
 
 
-_ops = None
-
-
 def _library():
-    """The package, imported at its first use."""
-    global _ops
-    if _ops is None:
-        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "qwen-drive-edge-orin_amd"))
-        import gdn_hip
+    pkg = str(Path(__file__).resolve().parents[1] / "qwen-drive-edge-orin_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    import gdn_hip
 
-        _ops = gdn_hip
-    return _ops
+    return gdn_hip
 
 
 def _silu(x):
