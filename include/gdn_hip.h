@@ -322,8 +322,8 @@ hipError_t gdn_ssm_step(const gdn_ssm_inputs* in, void* y, float* state, const i
 
 /* Prompts.  cu_seqlens null: `batch` sequences of `tokens` tokens (num_seqs is
  * batch).  cu_seqlens int32 [num_seqs + 1]: batch is 1 and the row holds
- * packed sequences (clamped as in deltanet_chunk_prefill_varlen; y rows behind
- * the last sequence are not written).  s0 (or null: zeros) and sf are fp32
+ * packed sequences (clamped as in deltanet_chunk_prefill_varlen; y rows in front
+ * of the first and behind the last sequence are not written).  s0 (or null: zeros) and sf are fp32
  * [num_seqs][heads][state_dim][head_dim], which must not overlap (a segment may
  * still read s0 when another one's end is written).  A sequence without tokens
  * hands its state on.  blocks (or null): gdn_request_blocks' table for
@@ -363,11 +363,10 @@ hipError_t gdn_request_blocks(const int32_t* lengths, const int32_t* slots, int 
  * fixed-length or packed sequences.  x, y, w, bias, K, dtypes and silu as
  * there; state0 (or null: zeros) and state are [num_seqs][D][state_len] of
  * io_dtype, oldest token first, state_len in K-1..8; states, w and bias are
- * 16-byte aligned; state
- * (out) holds the last state_len tokens of state0 followed by the sequence, and
- * must not be state0.  cu_seqlens (B = 1) as in gdn_ssm_scan, or null
- * (num_seqs is B); y rows behind the last sequence are not written.  The sum
- * stays in fp32 up to the one rounding of y. */
+ * 16-byte aligned; state (out) holds the last state_len tokens of state0
+ * followed by the sequence, and must not be state0.  cu_seqlens (B = 1) as in
+ * gdn_ssm_scan, or null (num_seqs is B).  The sum stays in fp32 up to the one
+ * rounding of y. */
 hipError_t gdn_causal_conv1d_prefill(const void* x, const void* w, const void* bias,
                                      const void* state0, void* y, void* state, int B, int T,
                                      int D, int K, int state_len, int64_t x_bstride,

@@ -13,8 +13,9 @@
 // anything is waited for; neighbouring runs share K - 1 rows (L2).  The
 // sequence of a run's first token comes from a search in cu_seqlens that
 // overlaps those loads (their addresses do not depend on it), and where a
-// run crosses into the next sequence the window is refilled from that
-// sequence's state, so that packed rows need neither padding nor a table.
+// run crosses into the next sequence (or into the first, where cu_seqlens does
+// not start at 0) the window is refilled from that sequence's state, so that
+// packed rows need neither padding nor a table.
 // The new states are formed by threads of their own behind the last run
 // (K rows each, in the cache), empty sequences among them.
 #include "gdn_common.h"
@@ -163,6 +164,7 @@ __global__ __launch_bounds__(kThreads) void causal_conv1d_prefill_kernel(const C
         lo = seq_lo(a.cu, 0, a.T, s);
         hi = lo + seq_count(a.cu, 0, a.T, s);
     }
+    int edge = t0 < lo ? lo : hi;   // the next token at which a sequence begins or ends
     auto state_tap = [&](int e, int back) {   // channel e of sequence s, `back` tokens before its first
         return a.state0 ? io_elem<IO>(a.state0, ((size_t)s * a.D + d0 + e) * a.L + a.L - back) : 0.f;
     };
@@ -185,16 +187,20 @@ __global__ __launch_bounds__(kThreads) void causal_conv1d_prefill_kernel(const C
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
         if (i >= len) return;
-        if (t0 + i >= hi) {   // into the next sequence that has tokens
-            do {
+        const int t = t0 + i;
+        if (t == edge) {
+            while (hi <= t) {   // into the next sequence that has tokens
                 if (++s >= a.seqs) return;
                 lo = seq_lo(a.cu, 0, a.T, s);
                 hi = lo + seq_count(a.cu, 0, a.T, s);
-            } while (hi <= t0 + i);
+            }
+            edge = t < lo ? lo : hi;
+            if (t >= lo) {
 #pragma unroll
-            for (int j = 0; j < K - 1; ++j) {
+                for (int j = 0; j < K - 1; ++j) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) win[j][e] = state_tap(e, K - 1 - j);
+                    for (int e = 0; e < 8; ++e) win[j][e] = state_tap(e, K - 1 - j);
+                }
             }
         }
 #pragma unroll
@@ -216,7 +222,8 @@ __global__ __launch_bounds__(kThreads) void causal_conv1d_prefill_kernel(const C
             }
             out[p] = io_pack<IO>(v[0], v[1]);
         }
-        __builtin_nontemporal_store(out, reinterpret_cast<u32x4*>(yb + (size_t)(t0 + i) * a.yts));
+        // (rows in front of the first sequence are no sequence's)
+        if (t >= lo) __builtin_nontemporal_store(out, reinterpret_cast<u32x4*>(yb + (size_t)t * a.yts));
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) {
 #pragma unroll
