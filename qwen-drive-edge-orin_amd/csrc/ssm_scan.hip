@@ -44,11 +44,11 @@
 // and d x, which enters the state, as three (fp32's 24 bits; two would leave
 // 2.4e-6 of the state).  fp16: pairs of fp16 behind a power-of-two scale that
 // fits them (22 bits).  Sums, states, decays:
-// fp32.  Logarithms are summed in fp32, forwards within 16 tokens for M and
-// backwards for the state's weights, so that the weights of the newest tokens,
-// the largest, are sums of few terms; a token's base-2 logarithm is held at
-// -150, where its decay is 0 in fp32, to keep the differences of M exact for
-// the tokens behind it.
+// fp32.  Logarithms are summed in fp32, backwards for the state's weights, so
+// that those of the newest tokens, the largest, are sums of few terms, and
+// forwards within 16 tokens for M, in two parts, so that differences of two
+// sums are as exact as the shorter sum; a token's base-2 logarithm is held at
+// -150, where its decay is 0 in fp32, to keep those sums small.
 #include "gdn_seq.h"
 #include "gdn_ssm.h"
 
@@ -299,11 +299,12 @@ struct Smem {
     uint16_t c[kLocal ? 8 : 64 * N];
     uint16_t x[WAVES][64 * 16 * PT];
     f32x4 cb[kLocal ? 1 : 10][64];   // (C B^T)^T tiles of the lower triangle, as fragments
-    // per token of the chunk, for each wave's head: the sum r of the log decays
-    // of its 16 up to it; the step d; the weight in S; d times the decay up to
-    // the end of its 16
+    // per token of the chunk, for each wave's head: the weight in S; the sum of
+    // the log decays of its 16 up to it, r in steps of 2^-8 and q the rest; the
+    // step d; d times the decay up to the end of its 16
+    static constexpr int kTok = kLocal ? 4 : 64;
     struct {
-        float r[64], d[64], w[64], f[64];
+        float w[64], r[kTok], q[kTok], d[kTok], f[kTok];
     } tok[WAVES];
 };
 
@@ -447,9 +448,12 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
     float d_max = 0.f, w_max = 0.f;
 
     // Token `lane` of a chunk of n: step, log decay, its sums.  They are kept
-    // by 16 tokens, with the sums of whole 16s apart: where strong decays
-    // (resets) and weak ones alternate, the difference of two sums over a whole
-    // chunk loses up to 7e-4 of a decay, that of two sums within 16 tokens 2e-4.
+    // by 16 tokens, with the sums of whole 16s apart, which are only ever added.
+    // Within 16 tokens M takes differences of two sums, and there a reset in
+    // front of both tokens must cost nothing: the sum up to a token is r + q, r
+    // the sum of the logarithms rounded to 2^-8 (at most 16 x 150 x 2^8 such
+    // steps: exact in fp32, and so are differences) and q that of what is left
+    // (below 2^-5, off by 2^-25).
     float sums[4];
     auto token_vectors = [&](float raw, int n) {
         const float d = lane < n ? ssm_delta(raw, bias, in.dt_min, in.dt_max) : 0.f;
@@ -467,7 +471,10 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
             w_max = wave_max(w);
         }
         if (!kLocal) {
-            tok.r[lane] = row_prefix(l2);
+            constexpr float kStep = 1.5f * 32768;   // fp32 is in steps of 2^-8 here
+            const float coarse = (l2 + kStep) - kStep;
+            tok.r[lane] = row_prefix(coarse);
+            tok.q[lane] = row_prefix(l2 - coarse);
             tok.d[lane] = d;
             tok.f[lane] = d * __builtin_amdgcn_exp2f(after);
         }
@@ -603,14 +610,11 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
                 k_m = fit_fp16(2.f * fmaxf(wave_max(top) * d_max, fabsf(D)));
                 Dm *= pow2(k_m);
             }
-            float ct[4];
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt) {
-                ct[tt] = tok.r[16 * tt + m];
                 const float before = tt == 0 ? 0.f : tt == 1 ? sums[0] : tt == 2 ? sums[0] + sums[1] : sums[0] + (sums[1] + sums[2]);
-                const float c = ct[tt] + before;
+                const float c = tok.r[16 * tt + m] + (tok.q[16 * tt + m] + before);
                 const float e = __builtin_amdgcn_exp2f(IO == 1 ? c + (float)(k_m - k_s - kappa) : c);
-                if (IO == 1) ct[tt] += (float)k_m;
 #pragma unroll
                 for (int pt = 0; pt < PT; ++pt) Y[pt][tt] *= e;
             }
@@ -619,6 +623,7 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
             // column and one per row, both at most 1.
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt) {
+                const float rt = tok.r[16 * tt + m] + (IO == 1 ? (float)k_m : 0.f), qt = tok.q[16 * tt + m];
 #pragma unroll
                 for (int kb = 0; kb <= tt / 2; ++kb) {
                     float v[8];
@@ -631,17 +636,18 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
                         } else if (st == tt) {
                             const f32x4 cb = sm.cb[tri(tt, st)][lane];
                             const f32x4 rs = *reinterpret_cast<const f32x4*>(tok.r + 16 * st + 4 * g);
+                            const f32x4 qs = *reinterpret_cast<const f32x4*>(tok.q + 16 * st + 4 * g);
                             const f32x4 ds = *reinterpret_cast<const f32x4*>(tok.d + 16 * st + 4 * g);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const float e = cb[i] * __builtin_amdgcn_exp2f(ct[tt] - rs[i]) * ds[i];
+                                const float e = cb[i] * __builtin_amdgcn_exp2f((rt - rs[i]) + (qt - qs[i])) * ds[i];
                                 v[4 * q + i] = (4 * g + i <= m ? e : 0.f) + Dm[i];
                             }
                         } else {
                             const f32x4 cb = sm.cb[tri(tt, st)][lane];
                             const f32x4 fs = *reinterpret_cast<const f32x4*>(tok.f + 16 * st + 4 * g);
                             const float between = tt - st == 1 ? 0.f : tt - st == 2 ? sums[st + 1] : sums[1] + sums[2];
-                            const float ht = __builtin_amdgcn_exp2f(ct[tt] + between);
+                            const float ht = __builtin_amdgcn_exp2f(rt + (qt + between));
 #pragma unroll
                             for (int i = 0; i < 4; ++i) v[4 * q + i] = cb[i] * (fs[i] * ht);
                         }
