@@ -42,9 +42,10 @@
 // Rounding.  bf16: x, B and C are exact operands; S and M = (C B^T) o decay
 // enter y's products as pairs of bf16 (2^-18 of each term, y itself has 2^-8),
 // and d x, which enters the state, as three (fp32's 24 bits; two would leave
-// 2.4e-6 of the state).  fp16: pairs of fp16 behind a power-of-two scale that
-// fits them (22 bits).  Sums, states, decays:
-// fp32.  Logarithms are summed in fp32, backwards for the state's weights, so
+// 2.4e-6 of the state).  fp16: pairs of fp16 (22 bits) behind powers of two, one
+// for each column of S and of w x, so that what is off is relative to a column's
+// own largest value, and one for M, off by 2^-40 of the chunk's largest
+// |C . B| d (y itself: 2^-11).  Sums, states, decays: fp32.  Logarithms are summed in fp32, backwards for the state's weights, so
 // that those of the newest tokens, the largest, are sums of few terms, and
 // forwards within 16 tokens for M, in two parts, so that differences of two
 // sums are as exact as the shorter sum; a token's base-2 logarithm is held at
@@ -131,6 +132,7 @@ __device__ __forceinline__ const uint16_t* piece_at(const uint16_t* base, int r,
     return base + (size_t)(r * PR + (p ^ swz<PR>(r))) * 8;
 }
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
@@ -282,6 +284,26 @@ __device__ __forceinline__ float wave_max(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
+// Two non-negative floats' upper halves in one word, x low (what fit_fp16 looks at)
+__device__ __forceinline__ uint32_t pack_tops(float x, float y) {
+    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302);
+}
+
+// Their maxima over the four lanes of a column (m, m + 16, m + 32 and m + 48)
+__device__ __forceinline__ uint32_t column_max(uint32_t v) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int off = 16; off < 64; off <<= 1)
+        v = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(
+                                             __builtin_bit_cast(u16x2, v),
+                                             __builtin_bit_cast(u16x2, (uint32_t)__shfl_xor((int)v, off, 64))));
+    return v;
+}
+
+__device__ __forceinline__ float top_of(uint32_t v, int i) {
+    return __builtin_bit_cast(float, i == 0 ? v << 16 : v & 0xffff0000u);
+}
+
 // k that brings x >= 0 into [2^14, 2^15), fp16's top binade but one; within
 // +-100, so that 2^k and a few sums of such k stay inside fp32's exponents
 __device__ __forceinline__ int fit_fp16(float x) {
@@ -305,7 +327,9 @@ struct Smem {
     static constexpr int kTok = kLocal ? 4 : 64;
     struct {
         float w[64], r[kTok], q[kTok], d[kTok], f[kTok];
+        int k[kLocal ? 4 : 16 * PT];   // fp16: the power of two on each column of S^T C^T
     } tok[WAVES];
+    alignas(16) float cb_top[WAVES];   // fp16: the largest of C B^T's column tile of each wave
 };
 
 __device__ __forceinline__ constexpr int tri(int tt, int st) { return tt * (tt + 1) / 2 + st; }
@@ -442,10 +466,36 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
     float log_total = 0.f;   // the segment's base-2 log decay
 
     // fp16: what enters an MFMA is scaled by a power of two first, so that
-    // neither large nor small values leave the five exponent bits.  The
-    // accumulators S hold 2^kappa times the state.
-    int kappa = 0;
-    float d_max = 0.f, w_max = 0.f;
+    // neither large nor small values leave the five exponent bits.  The state
+    // and w x have one for each column, so that a small channel next to a large
+    // one keeps its bits: the accumulators S hold 2^kappa times the state.
+    int kappa[PT];
+    float d_max = 0.f;
+    static_assert(PT == 2, "a word holds the maxima of a lane's columns, lane 16 pt + m keeps column m of tile pt");
+    auto column_tops = [&] {   // of S
+        float top[PT] = {0.f, 0.f};
+#pragma unroll
+        for (int pt = 0; pt < PT; ++pt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top[pt] = fmaxf(top[pt], fabsf(S[nt][pt][i]));
+        return column_max(pack_tops(top[0], top[1]));
+    };
+    auto scale_columns = [&](int sign) {
+#pragma unroll
+        for (int pt = 0; pt < PT; ++pt) {
+            const float f = pow2(sign * kappa[pt]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) S[nt][pt] *= f;
+        }
+    };
+    if constexpr (IO == 1) {
+        const uint32_t tops = column_tops();
+#pragma unroll
+        for (int pt = 0; pt < PT; ++pt) kappa[pt] = fit_fp16(top_of(tops, pt));
+        scale_columns(1);
+    }
 
     // Token `lane` of a chunk of n: step, log decay, its sums.  They are kept
     // by 16 tokens, with the sums of whole 16s apart, which are only ever added.
@@ -466,10 +516,7 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
         const float behind = g == 0 ? sums[1] + (sums[2] + sums[3]) : g == 1 ? sums[2] + sums[3] : g == 2 ? sums[3] : 0.f;
         const float w = d * __builtin_amdgcn_exp2f(after + behind);
         tok.w[lane] = w;
-        if (IO == 1) {
-            d_max = wave_max(d);
-            w_max = wave_max(w);
-        }
+        if (IO == 1) d_max = wave_max(d);
         if (!kLocal) {
             constexpr float kStep = 1.5f * 32768;   // fp32 is in steps of 2^-8 here
             const float coarse = (l2 + kStep) - kStep;
@@ -519,23 +566,22 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
         // From here to the barrier there is no branch: the token vectors' chain
         // of lane exchanges and C B^T's of LDS reads run beside S^T C^T
         token_vectors(raw, n);
-        float s_max = 0.f;
-        int k_s = 0;
-        if constexpr (IO == 1) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int pt = 0; pt < PT; ++pt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s_max = fmaxf(s_max, fabsf(S[nt][pt][i]));
-            s_max = wave_max(s_max);
-        }
+        uint32_t s_tops = 0;   // fp16: the largest of each column of S
+        if constexpr (IO == 1) s_tops = column_tops();
         if constexpr (!kLocal) {
             // (C B^T)^T: rows s, columns t of tile `wave` (of the tiles above the
             // diagonal, which nobody reads, too); S^T C^T: rows p, columns t
             static_assert(WAVES == 4, "a column tile of C B^T per wave");
-            if constexpr (IO == 1) k_s = fit_fp16(s_max);
-            const float s_scale = IO == 1 ? pow2(k_s) : 1.f;
+            float s_scale[PT];
+            if constexpr (IO == 1) {
+                int k_s[PT];
+#pragma unroll
+                for (int pt = 0; pt < PT; ++pt) {
+                    k_s[pt] = fit_fp16(top_of(s_tops, pt));
+                    s_scale[pt] = pow2(k_s[pt]);
+                }
+                if (g < PT) tok.k[lane] = g == 0 ? k_s[0] + kappa[0] : k_s[1] + kappa[1];
+            }
             f32x4 acc[4];
 #pragma unroll
             for (int st = 0; st < 4; ++st) acc[st] = zero4();
@@ -560,8 +606,8 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
                         v[i] = S[2 * kb][pt][i];
                         v[4 + i] = S[2 * kb + 1][pt][i];
                         if (IO == 1) {
-                            v[i] *= s_scale;
-                            v[4 + i] *= s_scale;
+                            v[i] *= s_scale[pt];
+                            v[4 + i] *= s_scale[pt];
                         }
                     }
                     s16x8 sop[2];
@@ -575,6 +621,15 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
 #pragma unroll
             for (int st = 0; st < 4; ++st)
                 if (st <= wave) sm.cb[tri(wave, st)][lane] = acc[st];
+            if constexpr (IO == 1) {   // (with what lies above the diagonal: a bound)
+                float top = 0.f;
+#pragma unroll
+                for (int st = 0; st < 4; ++st)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(acc[st][i]));
+                top = wave_max(top);
+                if (lane == 0) sm.cb_top[wave] = top;
+            }
         }
         s16x8 xop[PT][2];
 #pragma unroll
@@ -600,23 +655,26 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
             int k_m = 0;
             f32x4 Dm = Dd;
             if constexpr (IO == 1) {
-                float top = 0.f;
-#pragma unroll
-                for (int k = 0; k < 10; ++k) {
-                    const f32x4 cb = sm.cb[k][lane];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(cb[i]));
-                }
-                k_m = fit_fp16(2.f * fmaxf(wave_max(top) * d_max, fabsf(D)));
+                const f32x4 t = *reinterpret_cast<const f32x4*>(sm.cb_top);
+                const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+                k_m = fit_fp16(2.f * fmaxf(top * d_max, fabsf(D)));
+                k_m = __builtin_amdgcn_readfirstlane(k_m);
                 Dm *= pow2(k_m);
             }
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt) {
                 const float before = tt == 0 ? 0.f : tt == 1 ? sums[0] : tt == 2 ? sums[0] + sums[1] : sums[0] + (sums[1] + sums[2]);
                 const float c = tok.r[16 * tt + m] + (tok.q[16 * tt + m] + before);
-                const float e = __builtin_amdgcn_exp2f(IO == 1 ? c + (float)(k_m - k_s - kappa) : c);
+                const float e = __builtin_amdgcn_exp2f(c);
 #pragma unroll
-                for (int pt = 0; pt < PT; ++pt) Y[pt][tt] *= e;
+                for (int pt = 0; pt < PT; ++pt) {
+                    Y[pt][tt] *= e;
+                    if constexpr (IO == 1) {   // from its columns' scales to M's
+                        const i32x4 k = *reinterpret_cast<const i32x4*>(tok.k + 16 * pt + 4 * g);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) Y[pt][tt][i] = __builtin_ldexpf(Y[pt][tt][i], k_m - k[i]);
+                    }
+                }
             }
             // + X^T M^T, M[t][s] = (C B^T) e^{c_t - c_s} d_s for s <= t, + D for s = t.
             // Below the diagonal tiles the exponential is a product of one per
@@ -695,32 +753,45 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
 
         // S <- e^{c_Q} S + B^T (w x)
         const float total2 = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-        float dec = __builtin_amdgcn_exp2f(total2), w_scale = 1.f;
+        const float decay = __builtin_amdgcn_exp2f(total2);
         log_total += total2;
+        float dec[PT], w_scale[PT];
+        uint32_t wx_tops = 0;   // fp16: the largest of each column of w x
         if constexpr (IO == 1) {
-            // the new kappa: the larger of the decayed state and w x fits
-            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-            u16x2 top = {0, 0};
+            float top[PT] = {0.f, 0.f};
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int pt = 0; pt < PT; ++pt)
+                for (int q = 0; q < 2; ++q) {
+                    const f32x4 w = *reinterpret_cast<const f32x4*>(tok.w + 32 * kb + 16 * q + 4 * g);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        top = __builtin_elementwise_max(
-                            top, __builtin_bit_cast(u16x2, __builtin_bit_cast(u32x4, xop[pt][kb])[k] & 0x7fff7fffu));
-            const uint16_t xm = top[0] > top[1] ? top[0] : top[1];
-            const float wx_max = wave_max(fabsf((float)__builtin_bit_cast(_Float16, xm))) * w_max;
-            const int next_kappa = fit_fp16(fmaxf(dec * s_max * pow2(-kappa), wx_max));
-            // (a state that is 0 takes any scale, one 2^126 below w x is nothing)
-            dec = dec * s_max == 0.f ? 0.f : dec * pow2(min(max(next_kappa - kappa, -126), 127));
-            kappa = next_kappa;
-            w_scale = pow2(kappa);
+                    for (int pt = 0; pt < PT; ++pt)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const uint32_t xr = __builtin_bit_cast(u32x4, xop[pt][kb])[2 * q + k];
+                            top[pt] = fmaxf(fmaxf(top[pt], fabsf(io_lo<IO>(xr) * w[2 * k])),
+                                            fabsf(io_hi<IO>(xr) * w[2 * k + 1]));
+                        }
+                }
+            wx_tops = column_max(pack_tops(top[0], top[1]));
+        }
+#pragma unroll
+        for (int pt = 0; pt < PT; ++pt) {
+            dec[pt] = decay;
+            if constexpr (IO == 1) {
+                // the new kappa: the larger of the decayed state and w x fits
+                const float left = decay * top_of(s_tops, pt);
+                const int next_kappa = fit_fp16(fmaxf(left * pow2(-kappa[pt]), top_of(wx_tops, pt)));
+                // (a state that is 0 takes any scale)
+                dec[pt] = left == 0.f ? 0.f : __builtin_ldexpf(decay, next_kappa - kappa[pt]);
+                kappa[pt] = next_kappa;
+                w_scale[pt] = pow2(next_kappa);
+            }
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int pt = 0; pt < PT; ++pt) S[nt][pt] *= dec;
+            for (int pt = 0; pt < PT; ++pt) S[nt][pt] *= dec[pt];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             s16x8 wx[PT][kParts];
@@ -736,8 +807,8 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
                     v[2 * k] = io_lo<IO>(xr[k]) * w[2 * (k & 1)];
                     v[2 * k + 1] = io_hi<IO>(xr[k]) * w[2 * (k & 1) + 1];
                     if (IO == 1) {
-                        v[2 * k] *= w_scale;
-                        v[2 * k + 1] *= w_scale;
+                        v[2 * k] *= w_scale[pt];
+                        v[2 * k + 1] *= w_scale[pt];
                     }
                 }
                 split<IO, kParts>(v, wx[pt]);
@@ -753,13 +824,7 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
         }
     }
 
-    if constexpr (IO == 1) {
-        const float down = pow2(-kappa);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int pt = 0; pt < PT; ++pt) S[nt][pt] *= down;
-    }
+    if constexpr (IO == 1) scale_columns(-1);
     if (!store) return;
     if (kLocal) {
         f32x4* to = a.states + rec * (NT * PT * 64) + lane;

@@ -1,4 +1,5 @@
-"""The scan where decays of very different size meet."""
+"""The scan where values or decays of very different size meet: resets among
+weak decays, channels of mixed magnitude, states far from 1."""
 import pytest
 import torch
 
@@ -42,3 +43,51 @@ def test_resets_cost_no_precision(dev, dtype):
     half = torch.finfo(dtype).eps / 2
     tiny = torch.finfo(dtype).smallest_normal * half
     sc.close(oy, y, half * y.abs() + 2.0 ** -16.5 * (1 + half) * ya + tiny, f"resets {dtype} y")
+
+
+def test_fp16_large_steps_of_zeros(dev):
+    """Steps of 1e4 whose x is 0 leave the state of the other tokens exact."""
+    T = 640
+    d = sc.inputs(51, 1, T, 3, 64, 1, 64, HF, dt_dtype=torch.float32, z=False)
+    wipe = torch.rand(T, generator=torch.Generator().manual_seed(0)) < 0.5
+    d["dt"] = torch.where(wipe[None, :, None], torch.tensor(1e4), d["dt"] - 2)
+    d["x"] = torch.where(wipe[None, :, None, None], torch.zeros((), dtype=HF), d["x"])
+    for n in range(T - 6, T):   # the last token a reset, and not
+        e = {k: (v[:, :n] if k in ("x", "dt", "B", "C") else v) for k, v in d.items()}
+        y, S, ya, Sa = orc.ssm(**e)
+        print(f"large steps, {n} tokens", flush=True)
+        oy, oS = _scan(e, dev)
+        # (16 + L) 2^-22 of a term of decay e^-L, as above
+        sc.close(oS, S, 2.0 ** -17 * Sa + 1e-30, "large steps state")
+
+
+@pytest.mark.parametrize("N", [32, 64, 128, 256])
+@pytest.mark.parametrize("T", [20, 64, 150])
+def test_fp16_channels_of_mixed_magnitude(dev, T, N):
+    """Small channels next to an outlier keep every bit of their states: bounds
+    are elementwise, so each channel is held to its own size."""
+    d = sc.inputs(T, 1, T, 2, 96, 1, N, HF, z=False)
+    size = 10.0 ** (-3 + 3 * torch.rand(96, generator=torch.Generator().manual_seed(N)))
+    size[::13] = 1.5e4
+    d["x"] = (d["x"].float().clamp(-4, 4) * size).to(HF)
+    d["C"] = (d["C"].float() * 1e-3).to(HF)
+    d["D"] = d["D"] * 0
+    s0 = torch.randn(1, 2, N, 96, generator=torch.Generator().manual_seed(T)) * size
+    y, S, ya, Sa = orc.ssm(**d, s0=s0)
+    assert y.abs().max() < 6e4
+    print(f"mixed channels T={T} N={N}", flush=True)
+    oy, oS = _scan(d, dev, s0)
+    by, bS = sc.bounds(d, T, y, ya, Sa, HF)
+    sc.close(oS, S, bS, "mixed state")
+    sc.close(oy, y, by, "mixed y")
+
+
+def test_fp16_state_far_above_what_is_read(dev):
+    """A state of 2^50 that C never reads, and steps of 0: y is 0, not NaN."""
+    d = sc.inputs(3, 1, 70, 2, 64, 1, 64, HF, z=False)
+    d["dt"] = torch.full_like(d["dt"], -float("inf"))
+    d["C"] = torch.zeros_like(d["C"])
+    d["D"] = torch.zeros_like(d["D"])
+    s0 = 2.0 ** 50 * torch.randn(1, 2, 64, 64, generator=torch.Generator().manual_seed(1))
+    oy, oS = _scan(d, dev, s0)
+    assert (oy == 0).all() and torch.allclose(oS.cpu(), s0, rtol=2e-7)
