@@ -299,8 +299,11 @@ hipError_t gdn_causal_conv1d_update(const void* x, void* conv_state, const void*
  * below 2^24).  x, z, b, c
  * are 16-byte aligned with strides that are multiples of 8.  head_dim is a
  * multiple of 16 up to 256, state_dim 16, 32, 64, 128 or 256, 0 <= dt_min <=
- * dt_max.  A token whose inputs are not finite leaves undefined values in its
- * sequence from the 64-token chunk that holds it on. */
+ * dt_max.  Inputs that are not finite show where the formulas have them and in
+ * nothing else: x in its channel's y and state from its token on, B and dt in y
+ * and the states from their token on, C and z in their token's y, a state in
+ * its channels' y (infinities as infinities or NaN; a dt of -infinity is a step
+ * of 0). */
 typedef struct {
     const void *x, *dt, *b, *c, *z;
     const float *A_log, *D, *dt_bias;

@@ -45,11 +45,17 @@
 // 2.4e-6 of the state).  fp16: pairs of fp16 (22 bits) behind powers of two, one
 // for each column of S and of w x, so that what is off is relative to a column's
 // own largest value, and one for M, off by 2^-40 of the chunk's largest
-// |C . B| d (y itself: 2^-11).  Sums, states, decays: fp32.  Logarithms are summed in fp32, backwards for the state's weights, so
-// that those of the newest tokens, the largest, are sums of few terms, and
-// forwards within 16 tokens for M, in two parts, so that differences of two
-// sums are as exact as the shorter sum; a token's base-2 logarithm is held at
-// -150, where its decay is 0 in fp32, to keep those sums small.
+// |C . B| d (y itself: 2^-11).  Sums, states, decays: fp32.  Logarithms are
+// summed in fp32, backwards for the state's weights, so that those of the
+// newest tokens, the largest, are sums of few terms, and forwards within 16
+// tokens for M, in two parts, so that differences of two sums are as exact as
+// the shorter sum; a token's base-2 logarithm is held at -150, where its decay
+// is 0 in fp32, to keep those sums small.
+//
+// Not finite.  A product sums over the zeros of M too, and 0 x infinity would
+// reach tokens in front, so x that is not finite is 0 in the products and its
+// channel NaN from its token on.  4 MFMAs on zeros and a ballot find it, 0 to
+// 2 % of a call.  fp16's scales come from what is finite.
 #include "gdn_seq.h"
 #include "gdn_ssm.h"
 
@@ -156,6 +162,25 @@ __device__ __forceinline__ s16x8 tr_operand(const uint16_t* base, int t, int kb,
 template <int PR>
 __device__ __forceinline__ s16x8 row_operand(const uint16_t* base, int r, int p) {
     return *reinterpret_cast<const s16x8*>(piece_at<PR>(base, r, p));
+}
+
+// x that is not finite becomes 0 in a 64-row tile of 32 columns.  Lane's column
+// (lane % 32): the first row that had one, or 64.
+template <int IO, int PR>
+__device__ __forceinline__ int clear_not_finite(uint16_t* tile, int lane) {
+    static_assert(PR == 4, "32 columns, half of the rows a lane");
+    constexpr int kExp = IO == 0 ? 0x7f80 : 0x7c00;
+    int first = 64;
+#pragma unroll 1
+    for (int i = 31; i >= 0; --i) {
+        const int r = (lane & 32) + i;
+        uint16_t* at = const_cast<uint16_t*>(piece_at<PR>(tile, r, (lane & 31) / 8)) + lane % 8;
+        if ((*at & kExp) == kExp) {
+            first = r;
+            *at = 0;
+        }
+    }
+    return min(first, __shfl_xor(first, 32, 64));
 }
 
 template <int IO>
@@ -284,6 +309,9 @@ __device__ __forceinline__ float wave_max(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
+// x, or NaN for an infinity: the maxima that scales come from do not see NaN
+__device__ __forceinline__ float finite_or_nan(float x) { return fmaf(x, 0.f, x); }
+
 // Two non-negative floats' upper halves in one word, x low (what fit_fp16 looks at)
 __device__ __forceinline__ uint32_t pack_tops(float x, float y) {
     return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302);
@@ -328,6 +356,7 @@ struct Smem {
     struct {
         float w[64], r[kTok], q[kTok], d[kTok], f[kTok];
         int k[kLocal ? 4 : 16 * PT];   // fp16: the power of two on each column of S^T C^T
+        uint16_t first[kLocal ? 8 : 16 * PT];   // each column's first token whose x is not finite
     } tok[WAVES];
     alignas(16) float cb_top[WAVES];   // fp16: the largest of C B^T's column tile of each wave
 };
@@ -491,6 +520,13 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
         }
     };
     if constexpr (IO == 1) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int pt = 0; pt < PT; ++pt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    S[nt][pt][i] = finite_or_nan(S[nt][pt][i]);
         const uint32_t tops = column_tops();
 #pragma unroll
         for (int pt = 0; pt < PT; ++pt) kappa[pt] = fit_fp16(top_of(tops, pt));
@@ -516,7 +552,7 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
         const float behind = g == 0 ? sums[1] + (sums[2] + sums[3]) : g == 1 ? sums[2] + sums[3] : g == 2 ? sums[3] : 0.f;
         const float w = d * __builtin_amdgcn_exp2f(after + behind);
         tok.w[lane] = w;
-        if (IO == 1) d_max = wave_max(d);
+        if (IO == 1) d_max = wave_max(fmaxf(finite_or_nan(d), 0.f));
         if (!kLocal) {
             constexpr float kStep = 1.5f * 32768;   // fp32 is in steps of 2^-8 here
             const float coarse = (l2 + kStep) - kStep;
@@ -626,7 +662,7 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
 #pragma unroll
                 for (int st = 0; st < 4; ++st)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(acc[st][i]));
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(finite_or_nan(acc[st][i])));
                 top = wave_max(top);
                 if (lane == 0) sm.cb_top[wave] = top;
             }
@@ -636,6 +672,23 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int pt = 0; pt < PT; ++pt) xop[pt][kb] = tr_operand<XR>(xs, pt, kb, lane);
+        bool poisoned = false;   // main pass: x has values that are not finite
+        if constexpr (!kLocal) {
+            f32x4 none = zero4();
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int pt = 0; pt < PT; ++pt) none = mma<IO>(xop[pt][kb], s16x8{}, none);
+            poisoned = __any((none[0] + none[1]) + (none[2] + none[3]) != 0.f);
+            if (poisoned) {
+                const int first = clear_not_finite<IO, XR>(sm.x[wave], lane);
+                if (lane < 16 * PT) tok.first[lane] = (uint16_t)first;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int pt = 0; pt < PT; ++pt) xop[pt][kb] = tr_operand<XR>(xs, pt, kb, lane);
+            }
+        }
         __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): x is read
         __syncthreads();   // the vectors and C B^T are complete, C is read
         if (next > 0) {
@@ -725,6 +778,22 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
                 for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
                     for (int tt = 0; tt < 4; ++tt) Y[pt][tt] *= down;
+            }
+            if (poisoned) {   // (by integer masks: as many conditions would spill scalar registers)
+#pragma unroll
+                for (int pt = 0; pt < PT; ++pt) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int behind = tok.first[8 * g + 4 * pt + i] - m - 1;
+#pragma unroll
+                        for (int tt = 0; tt < 4; ++tt)
+                            Y[pt][tt][i] = __uint_as_float(__float_as_uint(Y[pt][tt][i]) |
+                                                           (uint32_t)((behind - 16 * tt) >> 31));
+                    }
+                    // and through w x the state
+                    const int own = tok.first[8 * (m >> 2) + 4 * pt + (m & 3)];
+                    xop[pt][0][0] = (short)(xop[pt][0][0] | (((own - kChunk) >> 31) & 0x7fff));
+                }
             }
             if (gate) {
 #pragma unroll

@@ -1,5 +1,6 @@
 """The scan where values or decays of very different size meet: resets among
-weak decays, channels of mixed magnitude, states far from 1."""
+weak decays, channels of mixed magnitude, states far from 1, and inputs that
+are not finite."""
 import pytest
 import torch
 
@@ -91,3 +92,88 @@ def test_fp16_state_far_above_what_is_read(dev):
     s0 = 2.0 ** 50 * torch.randn(1, 2, 64, 64, generator=torch.Generator().manual_seed(1))
     oy, oS = _scan(d, dev, s0)
     assert (oy == 0).all() and torch.allclose(oS.cpu(), s0, rtol=2e-7)
+
+
+BAD = [float("inf"), -float("inf"), float("nan")]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("N", [32, 128, 256])
+@pytest.mark.parametrize("bad", BAD)
+def test_x_not_finite(dev, bad, N, dtype):
+    """A value of x that is not finite shows in its channel from its token on,
+    and in nothing else: every other value is that of the call without it."""
+    for T, t, p in ((200, 41, 3), (200, 0, 63), (64, 63, 40), (500, 130, 17), (17, 16, 1)):
+        d = sc.inputs(T + t, 1, T, 2, 64, 1, N, dtype)
+        d["dt_bias"] = d["dt_bias"] - 3
+        d["x"] = d["x"].clone()
+        d["x"][0, t, 1, p] = 0
+        ry, rS = _scan(d, dev)
+        d["x"][0, t, 1, p] = bad
+        print(f"x {bad} at token {t} of {T}, N={N} {dtype}", flush=True)
+        oy, oS = _scan(d, dev)
+        assert not torch.isfinite(oy[0, t:, 1, p]).any() and not torch.isfinite(oS[0, 1, :, p]).any()
+        oy[0, t:, 1, p], oS[0, 1, :, p] = ry[0, t:, 1, p], rS[0, 1, :, p]
+        assert torch.equal(oy, ry) and torch.equal(oS, rS)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("bad", BAD)
+def test_others_not_finite(dev, bad, dtype):
+    """C and z: their token's y alone.  B and dt: y from its token on.  s0: its
+    channel's y.  Nothing in front, and no other channel."""
+    T, t = 150, 75
+    d = sc.inputs(6, 1, T, 2, 64, 1, 64, dtype)
+    d["dt_bias"] = d["dt_bias"] - 3
+    s0 = torch.randn(1, 2, 64, 64, generator=torch.Generator().manual_seed(1))
+    ry, rS = _scan(d, dev, s0)
+    step = torch.finfo(dtype).eps   # fp16: another scale of M, a rounding border away
+
+    def near(a, b):
+        assert torch.isfinite(a).all() and ((a.float() - b.float()).abs() <= step * (1 + b.float().abs())).all()
+
+    for k in ("C", "z", "B", "dt"):
+        e = dict(d)
+        e[k] = d[k].clone()
+        e[k][(0, t, 0, 5)[:d[k].dim()] if k != "dt" else (0, t, 1)] = bad
+        print(f"{k} {bad} {dtype}", flush=True)
+        if k == "dt" and bad == -float("inf"):
+            continue   # a step of 0
+        oy, oS = _scan(e, dev, s0)
+        if k == "C":
+            assert not torch.isfinite(oy[0, t]).any()
+            oy[0, t] = ry[0, t]
+        elif k == "z":
+            assert not torch.isfinite(oy[0, t, 0, 5])
+            oy[0, t, 0, 5] = ry[0, t, 0, 5]
+        elif k == "B":
+            assert not torch.isfinite(oy[0, t:]).any() and not torch.isfinite(oS[0, :, 5]).any()
+            oy[0, t:], oS = ry[0, t:], rS
+        else:
+            assert not torch.isfinite(oy[0, t:, 1]).any() and not torch.isfinite(oS[0, 1]).any()
+            oy[0, t:, 1], oS[0, 1] = ry[0, t:, 1], rS[0, 1]
+        near(oy, ry)
+        assert torch.allclose(oS, rS, rtol=1e-5, atol=1e-5)
+    s = s0.clone()
+    s[0, 1, 7, 9] = bad
+    oy, oS = _scan(d, dev, s)
+    assert not torch.isfinite(oy[0, :, 1, 9]).any() and not torch.isfinite(oS[0, 1, 7, 9])
+    oy[0, :, 1, 9], oS[0, 1, 7, 9] = ry[0, :, 1, 9], rS[0, 1, 7, 9]
+    assert torch.equal(oy, ry) and torch.equal(oS, rS)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_x_not_finite_in_a_split_sequence(dev, dtype):
+    """Through the first pass, its records and their join."""
+    T, t = 1250, 300
+    assert gdn_hip.ssm_scan_block(T, 1, 2, 64, 1, 64, 1) == 64
+    d = sc.inputs(8, 1, T, 2, 64, 1, 64, dtype)
+    d["dt_bias"] = d["dt_bias"] - 3
+    d["x"] = d["x"].clone()
+    d["x"][0, t, 1, 7] = 0
+    ry, rS = _scan(d, dev)
+    d["x"][0, t, 1, 7] = float("inf")
+    oy, oS = _scan(d, dev)
+    assert not torch.isfinite(oy[0, t:, 1, 7]).any() and not torch.isfinite(oS[0, 1, :, 7]).any()
+    oy[0, t:, 1, 7], oS[0, 1, :, 7] = ry[0, t:, 1, 7], rS[0, 1, :, 7]
+    assert torch.equal(oy, ry) and torch.equal(oS, rS)
