@@ -11,8 +11,11 @@
 // Runs of `block` tokens (segments) are worked on side by side: a first pass
 // forms each segment's state from zero (from s0 for a sequence's first one;
 // the last segment needs none), a join turns those into the states in front
-// of the segments, and the main pass starts each segment from its own.  A
-// call whose sequences have one segment each runs the main pass alone.
+// of the segments, and the main pass starts each segment from its own.  A call
+// that no sequence of which can be split runs the main pass alone (a packed one
+// where all its tokens fit in a block: the lengths are on the GPU).  Only
+// segments with another behind them have a record: 1500 requests, nearly all
+// single tokens, x 64 heads take 4 MB of workspace, not 3 GB.
 //
 // A wave owns 32 columns of one head: its slice of S stays in fp32 accumulators
 // through the segment, and the columns need nothing from one another.  Four
@@ -83,6 +86,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct Seg {
     int seq, t0, n, idx;
+    int rec;      // its record's place (the last of a sequence has none); the one in front is rec - 1
     bool last;
 };
 
@@ -93,14 +97,15 @@ struct ScanArgs {
     float* sf;
     const int4* table;   // packed: blocks; null: `segs` segments of `block` tokens per batch row
     int rows;            // segments (bound)
+    int recs;            // records: segments that are not the last of their sequence (bound)
     int segs, seqs, block;
     int slices;          // column slices of a head: ceil(P / PW)
     int tasks;           // slices of a group: heads / groups x slices
     bool fold;           // the main pass joins the segments' states itself
     int quads;           // work-groups per group and segment: ceil(tasks / waves)
     int* order;          // the main pass's rows, longest first; null: as they lie
-    f32x4* states;       // [row][group][task] fragments of a slice's state
-    float* decays;       // [row][group][task]
+    f32x4* states;       // [record][group][task] fragments of a slice's state
+    float* decays;       // [record][group][task]
 };
 
 // Segment r, clamped so that whatever a table holds its tokens lie in the row
@@ -110,15 +115,19 @@ __device__ __forceinline__ bool segment(const ScanArgs& a, int r, Seg& s) {
         s.idx = r - s.seq * a.segs;
         s.t0 = s.idx * a.block;
         s.n = min(a.block, a.in.tokens - s.t0);
+        s.rec = s.seq * (a.segs - 1) + s.idx;
         s.last = s.idx + 1 == a.segs;
         return true;
     }
+    // Records of packed segments lie at first token / block: a segment that is
+    // not its sequence's last is `block` tokens long, and no two overlap.
     const int4 b = a.table[r];
     if (b.x < 0 || b.x >= a.seqs) return false;
     s.seq = b.x;
     s.t0 = min(max(b.y, 0), a.in.tokens);
     s.n = min(min(max(b.z, 0), a.block), a.in.tokens - s.t0);
-    s.idx = b.w > 0 && r > 0 ? b.w : 0;
+    s.rec = min(s.t0 / a.block, a.recs);
+    s.idx = s.rec > 0 ? max(b.w, 0) : 0;
     s.last = r + 1 >= a.rows || a.table[r + 1].x != b.x;
     return true;
 }
@@ -403,7 +412,7 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
         else if (grp == 0 && quad == 0) order_row(a, row);
     }
     Seg s;
-    if (row >= a.rows || !segment(a, row, s) || (kLocal && s.last)) return;
+    if (row >= a.rows || !segment(a, row, s) || (kLocal && (s.last || s.rec >= a.recs))) return;
     const int task = quad * WAVES + wave;
     const bool store = task < a.tasks;   // waves past the group's last slice repeat it
     const int tk = min(task, a.tasks - 1);
@@ -453,7 +462,7 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
 #pragma unroll
         for (int pt = 0; pt < PT; ++pt) S[nt][pt] = zero4();
     const size_t hs = ((size_t)s.seq * H + h) * N * P;
-    const int64_t rec = ((int64_t)row * in.groups + grp) * a.tasks + tk;   // state record
+    const int64_t rec = ((int64_t)s.rec * in.groups + grp) * a.tasks + tk;   // state record
     // element (nt, pt, i) of a lane in a state [N][P]: so + n_off(nt, i) P + p_off(pt)
     const size_t so = hs + (size_t)(8 * g) * P + p0 + 8 * (m >> 2) + (m & 3);
     auto n_off = [](int nt, int i) { return 32 * (nt >> 1) + 4 * (nt & 1) + i; };
@@ -924,17 +933,24 @@ template <typename V>
 __global__ __launch_bounds__(kThreads) void ssm_join_kernel(const ScanArgs a, int elems, int parts) {
     const int64_t all = (int64_t)a.in.groups * a.tasks;   // records of a segment
     const int part = blockIdx.x % parts, rest = blockIdx.x / parts;
-    const int rec = rest % (int)all, seq = rest / (int)all;
-    int row = seq * a.segs, count = a.segs;   // the sequence's first segment, and how many
+    const int rec = rest % (int)all, nth = rest / (int)all;
+    int first = nth * (a.segs - 1), count = a.segs;   // a sequence's first record, and its segments
     if (a.table) {
-        int lo = 0, hi = a.rows;   // (-1 behind the last block is past every sequence)
+        // packed: sequence nth, or where those outnumber the records the one that
+        // begins at record nth: its row is the last in front of the next record's
+        const bool by_seq = a.seqs < a.recs;
+        int lo = 0, hi = a.rows;   // (rows behind the last block are -1)
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if ((unsigned)a.table[mid].x >= (unsigned)seq) hi = mid;
+            const int4 b = a.table[mid];
+            if (b.x < 0 || (by_seq ? b.x >= nth : b.y >= (nth + 1) * a.block)) hi = mid;
             else lo = mid + 1;
         }
-        row = lo;
-        if (row >= a.rows || a.table[row].x != seq) return;
+        const int row = by_seq ? lo : lo - 1;
+        if (row < 0 || row + 2 >= a.rows) return;
+        const int4 b = a.table[row];
+        const int seq = b.x;
+        if ((by_seq && seq != nth) || b.w != 0 || a.table[row + 2].x != seq) return;
         for (int base = row;; base += 64) {
             const int r = base + (threadIdx.x & 63);
             const unsigned long long other = __ballot(r >= a.rows || a.table[min(r, a.rows - 1)].x != seq);
@@ -943,11 +959,13 @@ __global__ __launch_bounds__(kThreads) void ssm_join_kernel(const ScanArgs a, in
                 break;
             }
         }
+        first = min(max(b.y, 0) / a.block, a.recs);
+        count = min(count, a.recs - first + 1);   // (as it is, for a table of this batch)
     }
     const int e = part * kThreads + threadIdx.x;
     if (count < 3 || e >= elems) return;
-    V* const at = reinterpret_cast<V*>(a.states) + (row * all + rec) * elems + e;
-    const float* const decay = a.decays + row * all + rec;
+    V* const at = reinterpret_cast<V*>(a.states) + (first * all + rec) * elems + e;
+    const float* const decay = a.decays + first * all + rec;
     const int64_t step = all * elems;
     constexpr int kAhead = 8;
     V R = at[0];
@@ -1061,7 +1079,7 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 struct Layout {
     int segs;        // segments of a batch row (0: packed)
-    int64_t rows;
+    int64_t rows, recs;
     int slices, tasks, quads;
     bool ordered;
     size_t table, starts, order, states, decays, total;   // byte offsets
@@ -1072,20 +1090,22 @@ struct Layout {
         slices = (in->head_dim + kCols - 1) / kCols;
         tasks = in->heads / in->groups * slices;
         quads = (tasks + kWaves - 1) / kWaves;
+        // a record for each segment but the last of a sequence: packed, whole
+        // blocks with a token behind them (the recurrence needs none, and no table)
+        recs = !chunked(in) ? 0 : packed ? std::max(in->tokens - 1, 0) / block : (int64_t)(segs - 1) * seqs;
         size_t off = 0;
         table = off;
-        if (packed) off += align256((size_t)rows * 16);
+        if (packed && chunked(in)) off += align256((size_t)rows * 16);
         starts = off;
-        if (packed) off += align256(((size_t)seqs + 1) * 4);
+        if (packed && chunked(in)) off += align256(((size_t)seqs + 1) * 4);
         order = off;
-        ordered = packed && rows * in->groups * quads <= kMaxOrder;
+        ordered = packed && recs > 0 && rows * in->groups * quads <= kMaxOrder;
         if (ordered) off += align256((size_t)rows * 4);
-        // no states where every sequence is one segment
-        const size_t recs = packed || segs > 1 ? (size_t)rows * in->groups * tasks : 0;
+        const size_t states_of = (size_t)recs * in->groups * tasks;
         states = off;
-        off += align256(recs * in->state_dim * kCols * 4);
+        off += align256(states_of * in->state_dim * kCols * 4);
         decays = off;
-        off += align256(recs * 4);
+        off += align256(states_of * 4);
         total = std::max<size_t>(off, 256);
     }
 };
@@ -1094,15 +1114,16 @@ template <int IO, int N, int PT, int WAVES>
 hipError_t launch_scan(const ScanArgs& a, hipStream_t stream) {
     const int64_t groups = ((int64_t)a.rows * a.in.groups + 7) / 8 * 8 * a.quads;
     if (groups > 0x7fffffff) return hipErrorInvalidValue;
-    if (a.table || a.segs > 1) {
+    if (a.recs > 0) {
         hipLaunchKernelGGL((ssm_scan_kernel<IO, N, PT, WAVES, true>), dim3((unsigned)groups),
                            dim3(64 * WAVES), 0, stream, a);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-        if (a.table || a.segs > kMaxFold) {
+        if (a.table ? a.recs > 1 : a.segs > kMaxFold) {
             // 16 bytes a thread from 2^17 such threads on (8 sequences of 2..7
             // segments x 128 records: 13 us against 35 with 4 bytes; one of 64
             // segments x 32 records: 30 us against 15)
-            const int64_t records = (int64_t)a.seqs * a.in.groups * a.tasks;
+            const int64_t all = (int64_t)a.in.groups * a.tasks;
+            const int64_t records = (a.table ? std::min(a.seqs, a.recs) : a.seqs) * all;
             const bool wide = records * N * PT * 4 >= 1 << 17;
             const int elems = N * PT * (wide ? 4 : 16), parts = (elems + kThreads - 1) / kThreads;
             if (records * parts > 0x7fffffff) return hipErrorInvalidValue;
@@ -1245,6 +1266,7 @@ extern "C" hipError_t gdn_ssm_scan(const gdn_ssm_inputs* in, void* y, const floa
     a.s0 = s0;
     a.sf = sf;
     a.rows = (int)l.rows;
+    a.recs = (int)l.recs;
     a.segs = l.segs;
     a.seqs = num_seqs;
     a.block = block;
