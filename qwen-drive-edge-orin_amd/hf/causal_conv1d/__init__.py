@@ -64,11 +64,17 @@ def causal_conv1d_fn(x, weight, bias=None, seq_idx=None, initial_states=None,
     if seq_idx is not None:
         raise NotImplementedError("seq_idx is not supported")
     silu = _silu(activation)
-    _on_device(x=x, weight=weight, bias=bias, initial_states=initial_states,
-               final_states_out=final_states_out)
+    if final_states_out is not None and not return_final_states:
+        raise ValueError("final_states_out goes with return_final_states=True")
     if x.dim() != 3:
         raise ValueError("x must be [B, D, T]")
     weight = _weight(weight)
+    states = (x.shape[0], x.shape[1], weight.shape[1] - 1)
+    for name, t in (("initial_states", initial_states), ("final_states_out", final_states_out)):
+        if t is not None and tuple(t.shape) != states:
+            raise ValueError(f"{name} must be [B, D, K - 1], here {list(states)}")
+    _on_device(x=x, weight=weight, bias=bias, initial_states=initial_states,
+               final_states_out=final_states_out)
     if initial_states is None and not return_final_states:
         return gdn_hip.causal_conv1d_fwd(x, weight, bias, silu)
     y, final = gdn_hip.causal_conv1d_prefill(x, weight, bias, initial_states, silu=silu,
