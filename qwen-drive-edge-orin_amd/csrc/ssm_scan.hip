@@ -42,12 +42,15 @@
 // interleaved by quarters of the chunk (spills), 8-wave groups, operand
 // residuals by dot products.
 //
-// Rounding.  bf16: x, B and C are exact operands; S and M = (C B^T) o decay
-// enter y's products as pairs of bf16 (2^-18 of each term, y itself has 2^-8),
-// and d x, which enters the state, as three (fp32's 24 bits; two would leave
-// 2.4e-6 of the state).  fp16: pairs of fp16 (22 bits) behind powers of two, one
-// for each column of S and of w x, so that what is off is relative to a column's
-// own largest value, and one for M, off by 2^-40 of the chunk's largest
+// Rounding.  bf16: x, B and C are exact operands.  M = (C B^T) o decay, which
+// carries D and the newest tokens, the largest terms of y, and d x, which enters
+// the state, go into products as three bf16 (fp32's 24 bits).  S enters y's
+// product as two, 2^-18 of each term, where C has 2^-9 already: M as two put
+// 1.2e-4 of y (its norm) on the other side of a bf16 border than fp32 does, as
+// three 2.2e-5 for 2 to 3 % of a call; S as three left that as it was for 4 to
+// 6 % more.  fp16: pairs of fp16 (22 bits) behind powers of two, one for each
+// column of S and of w x, so that what is off is relative to a column's own
+// largest value, and one for M, off by 2^-40 of the chunk's largest
 // |C . B| d (y itself: 2^-11).  Sums, states, decays: fp32.  Logarithms are
 // summed in fp32, backwards for the state's weights, so that those of the
 // newest tokens, the largest, are sums of few terms, and forwards within 16
@@ -393,7 +396,7 @@ __device__ __forceinline__ void order_row(const ScanArgs& a, int r) {
 template <int IO, int N, int PT, int WAVES, bool kLocal>
 __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(const ScanArgs a) {
     constexpr int NT = N / 16, NKB = N / 32, PR = N / 8, XR = 2 * PT, PW = 16 * PT;
-    constexpr int kParts = IO == 0 ? 3 : 2;   // of w x: 24 or 22 bits
+    constexpr int kParts = IO == 0 ? 3 : 2;   // of w x and M: 24 or 22 bits
     __shared__ Smem<N, PT, WAVES, kLocal> sm;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -772,10 +775,10 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
                             for (int i = 0; i < 4; ++i) v[4 * q + i] = cb[i] * (fs[i] * ht);
                         }
                     }
-                    s16x8 mop[2];
-                    split<IO, 2>(v, mop);
+                    s16x8 mop[kParts];
+                    split<IO, kParts>(v, mop);
 #pragma unroll
-                    for (int k = 1; k >= 0; --k)
+                    for (int k = kParts - 1; k >= 0; --k)
 #pragma unroll
                         for (int pt = 0; pt < PT; ++pt) Y[pt][tt] = mma<IO>(xop[pt][kb], mop[k], Y[pt][tt]);
                 }

@@ -62,6 +62,23 @@ def test_fp16_large_steps_of_zeros(dev):
         sc.close(oS, S, 2.0 ** -17 * Sa + 1e-30, "large steps state")
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_d_x_is_rounded_once(dev, dtype):
+    """With C = 0, y is D x: rounded to the type as the 64-bit product is, wherever
+    that lies further from a border than what three bf16 parts of D (2^-24) and
+    two sums in fp32 are off, or two fp16 parts (2^-22): 2^-21 and 2^-20 of it."""
+    d = sc.inputs(5, 1, 300, 512, 16, 1, 32, dtype, z=False)   # many values of D
+    d["C"] = torch.zeros_like(d["C"])
+    print(f"D x {dtype}", flush=True)
+    oy, _ = _scan(d, dev)
+    y = d["D"].double()[:, None] * d["x"].double()
+    away = 2.0 ** (-21 if dtype == BF else -20) * y.abs()
+    clear = (y - away).to(dtype) == (y + away).to(dtype)
+    clear &= y.abs() > torch.finfo(dtype).smallest_normal   # (below, fp16 is in steps of 2^-24)
+    assert clear.double().mean() > 0.99
+    assert torch.equal(oy.cpu()[clear], y.to(dtype)[clear])
+
+
 @pytest.mark.parametrize("N", [32, 64, 128, 256])
 @pytest.mark.parametrize("T", [20, 64, 150])
 def test_fp16_channels_of_mixed_magnitude(dev, T, N):
