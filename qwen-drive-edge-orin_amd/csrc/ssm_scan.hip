@@ -32,15 +32,18 @@
 // consecutive channels (perm below), 16 bytes of y.
 //
 // Measured (state 128): 8 packed prompts, 19,861 tokens x 64 heads of 64 with
-// the gate: 296 us, 2.0 TB/s of what must move: main pass 220, first pass 81,
-// join 15, table 3.  16,384 tokens x 16 heads 74 us, 1141 x 64 37 us.  In the
-// main pass the SIMDs issue vector instructions 49 % of the time and the MFMA
-// units are busy 26 % (0.6 PFLOP/s): two waves a SIMD, each in order, with a
-// seventh of the products for operands' second and third parts and M's
-// exponentials, splits and the gate on the vector units.  Measured without
-// gain: waves' priorities raised in the MFMA or the vector phases, update and M
-// interleaved by quarters of the chunk (spills), 8-wave groups, operand
-// residuals by dot products.
+// the gate: a call of 303 us, 2.0 TB/s of what must move; traced, where kernels
+// do not run into one another, main pass 225, first pass 65, join 16, table 5.
+// 16,384 tokens x 16 heads 78 us, 1141 x 64 38 us.  No unit is at its limit in
+// the main pass: the SIMDs issue vector instructions 52 % of the time and the
+// MFMA units are busy 27 % (0.6 PFLOP/s).  A wave runs in order and there are
+// two a SIMD: of a wave's time 43 % is its own issue, 34 % the other's turn and
+// 23 % a wait for memory, LDS or the barrier.  A wave's chunk takes 1,600 vector
+// instructions, 216 of them MFMA, the rest the splits of operands into parts,
+// M's exponentials (M is formed once per 32 columns, by each wave of a head) and
+// the gate.  Measured without gain: waves' priorities raised in the MFMA or the
+// vector phases, update and M interleaved by quarters of the chunk (spills),
+// 8-wave groups, operand residuals by dot products.
 //
 // Rounding.  bf16: x, B and C are exact operands.  M = (C B^T) o decay, which
 // carries D and the newest tokens, the largest terms of y, and d x, which enters
@@ -75,11 +78,12 @@ constexpr int kMaxBlock = 1 << 20;
 // Segments of a fixed-length sequence that the main pass joins by itself: each
 // group reads the records in front of its own, which is less than a launch of
 // the join up to here (1141 tokens x 64 heads in 6 segments: 38 us against 41;
-// 4 x 2048 tokens x 32 in 8: 95 against 82)
+// 4 x 2048 tokens x 32 in 8: 85 against 83)
 constexpr int kMaxFold = 6;
 // Work-groups of a packed call up to which the main pass takes the longest
 // segments first (8 rounds of 512: what the last round wastes still counts
-// against a group's one more trip to memory)
+// against a group's one more trip to memory; 30 prompts of 50 to 2000 tokens x
+// 64 heads 346 us against 371 in the table's order)
 constexpr int kMaxOrder = 4096;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
@@ -692,7 +696,7 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
 #pragma unroll
                 for (int pt = 0; pt < PT; ++pt) none = mma<IO>(xop[pt][kb], s16x8{}, none);
             poisoned = __any((none[0] + none[1]) + (none[2] + none[3]) != 0.f);
-            if (poisoned) {
+            if (__builtin_expect(poisoned, 0)) {
                 const int first = clear_not_finite<IO, XR>(sm.x[wave], lane);
                 if (lane < 16 * PT) tok.first[lane] = (uint16_t)first;
 #pragma unroll
@@ -791,7 +795,7 @@ __global__ __launch_bounds__(64 * WAVES, N > 128 ? 1 : 2) void ssm_scan_kernel(c
 #pragma unroll
                     for (int tt = 0; tt < 4; ++tt) Y[pt][tt] *= down;
             }
-            if (poisoned) {   // (by integer masks: as many conditions would spill scalar registers)
+            if (__builtin_expect(poisoned, 0)) {   // (by integer masks: as many conditions would spill scalar registers)
 #pragma unroll
                 for (int pt = 0; pt < PT; ++pt) {
 #pragma unroll
@@ -1188,17 +1192,17 @@ static double passes_us(double groups, double chunks, int deep, const double* t,
 // to 64 KB a record and pass).  The constants are measured at state_dim 128
 // (main pass: 5.7 and 8.8 us a chunk with one and two groups on a CU; first pass
 // 2.9, 3.3 and 3.6 with one to three; about 5 us to start a group from its
-// state), the rule's choices at most 11 % slower than the best of 1 .. 256
-// chunks over 23 calls (77 to 65,536 tokens, 8 to 128 heads, 1 to 101 sequences),
-// 2 % on average.
+// state), the rule's choices 1 % slower on average than the best of 1 .. 256
+// chunks over 23 calls (130 to 65,536 tokens, 8 to 128 heads, 1 to 101
+// sequences), at most 15 % (130 tokens x 64 heads, 3 chunks 20.6 us against 17.8).
 //
 // A packed batch whose sequences fill the chip 1.2 times without a split is
 // split only where one would hold the others up: at 1.5 times the chunks that
-// a place then works off (30 prompts of 50 to 2000 tokens x 64 heads: 331 us
-// against 442 by the estimate above).  The lengths are on the GPU, so what a
-// packed call takes is a guess: over 192 batches (2 to 64 prompts, uniform
-// lengths, and one long among short ones) the choices are 4 % slower on average
-// than the best, at most 37 %.
+// a place then works off (30 prompts of 50 to 2000 tokens x 64 heads: 47 chunks
+// 336 us against 449 at the estimate's 8).  The lengths are on the GPU, so what a
+// packed call takes is a guess: over 37 batches (2 to 300 prompts, uniform
+// lengths, and one long among short ones) the choices are 5 % slower on average
+// than the best, at most 33 %.
 extern "C" int gdn_ssm_scan_block(const gdn_ssm_inputs* in, int num_seqs) {
     if (!ssm_sizes_ok(in) || num_seqs < 1 || in->tokens > (1 << 30)) return 0;
     const int tasks = in->heads / in->groups * ((in->head_dim + kCols - 1) / kCols);
