@@ -296,14 +296,17 @@ hipError_t gdn_causal_conv1d_update(const void* x, void* conv_state, const void*
  *   A_log: fp32 [heads]; D, dt_bias: fp32 [heads] or null (zeros)
  * A row's heads (groups) lie next to each other; batches and tokens lie
  * *_batch and *_token elements apart (token strides, and heads x head_dim,
- * below 2^24).  x, z, b, c
- * are 16-byte aligned with strides that are multiples of 8.  head_dim is a
- * multiple of 16 up to 256, state_dim 16, 32, 64, 128 or 256, 0 <= dt_min <=
- * dt_max.  Inputs that are not finite show where the formulas have them and in
- * nothing else: x in its channel's y and state from its token on, B and dt in y
- * and the states from their token on, C and z in their token's y, a state in
- * its channels' y (infinities as infinities or NaN; a dt of -infinity is a step
- * of 0). */
+ * below 2^24).  x, z, b, c are 16-byte aligned with strides that are multiples
+ * of 8.  head_dim is a multiple of 16 up to 256, state_dim 16, 32, 64, 128 or
+ * 256, 0 <= dt_min <= dt_max.
+ * Sums, states and decays are fp32; y is rounded once.  In prompts, S enters
+ * y's product with 2^-18 of each term off in bf16, 2^-22 of its channel's
+ * largest in fp16.
+ * Inputs that are not finite show where the formulas have them and in nothing
+ * else: x in its channel's y and state from its token on, B and dt in y and the
+ * states from their token on, C and z in their token's y, a state in its
+ * channels' y (infinities as infinities or NaN; a dt of -infinity is a step of
+ * 0). */
 typedef struct {
     const void *x, *dt, *b, *c, *z;
     const float *A_log, *D, *dt_bias;
@@ -326,12 +329,12 @@ hipError_t gdn_ssm_step(const gdn_ssm_inputs* in, void* y, float* state, const i
 /* Prompts.  cu_seqlens null: `batch` sequences of `tokens` tokens (num_seqs is
  * batch).  cu_seqlens int32 [num_seqs + 1]: batch is 1 and the row holds
  * packed sequences (clamped as in deltanet_chunk_prefill_varlen; y rows in front
- * of the first and behind the last sequence are not written).  s0 (or null: zeros) and sf are fp32
- * [num_seqs][heads][state_dim][head_dim], which must not overlap (a segment may
- * still read s0 when another one's end is written).  A sequence without tokens
- * hands its state on.  blocks (or null): gdn_request_blocks' table for
- * the same cu_seqlens and this `block`; without it a packed call forms the
- * table itself in the workspace.  `block` is the run of tokens that is worked
+ * of the first and behind the last sequence are not written).  s0 (or null:
+ * zeros) and sf are fp32 [num_seqs][heads][state_dim][head_dim], which must not
+ * overlap (a segment may still read s0 when another one's end is written).  A
+ * sequence without tokens hands its state on.  blocks (or null):
+ * gdn_request_blocks' table for the same cu_seqlens and this `block`; without it
+ * a packed call forms the table itself in the workspace.  `block` is the run of tokens that is worked
  * on at a time, a multiple of 64, normally gdn_ssm_scan_block's; results for
  * different blocks differ by rounding.  The workspace is 256-byte aligned,
  * gdn_ssm_scan_workspace_size bytes (0: unsupported arguments). */
