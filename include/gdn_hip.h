@@ -299,9 +299,9 @@ hipError_t gdn_causal_conv1d_update(const void* x, void* conv_state, const void*
  * below 2^24).  x, z, b, c are 16-byte aligned with strides that are multiples
  * of 8.  head_dim is a multiple of 16 up to 256, state_dim 16, 32, 64, 128 or
  * 256, 0 <= dt_min <= dt_max.
- * Sums, states and decays are fp32; y is rounded once.  In prompts, S enters
- * y's product with 2^-18 of each term off in bf16, 2^-22 of its channel's
- * largest in fp16.
+ * Sums, states and decays are fp32; y is rounded once.  What enters y's products
+ * in prompts is off by 2^-18 of each term of S in bf16; in fp16 by 2^-22 of a
+ * channel's largest S and 2^-40 of the largest |C . B| d among 64 tokens.
  * Inputs that are not finite show where the formulas have them and in nothing
  * else: x in its channel's y and state from its token on, B and dt in y and the
  * states from their token on, C and z in their token's y, a state in its
